@@ -266,6 +266,99 @@ int qasr_final_norm_lmhead_argmax_noalloc(int32_t *ids_out, float *logits_out, c
                                           float eps, void *stream);
 
 /* ======================================================================
+ * Serving operators: INT8 KV cache, attention over it, token picks
+ * ==================================================================== */
+
+/* A KV cache of one byte per value (no counterpart in the reference, whose
+ * KvCache is f32: decoder.rs:130-202).  Codes [n_slots, n_layers, max_seq,
+ * n_kv_heads * head_dim] and one f32 scale per head of every row [n_slots,
+ * n_layers, max_seq, n_kv_heads], all on one device; value = code * scale.
+ * k and v 16-byte aligned; head_dim 64 or 128; n_kv_heads <= 256. */
+typedef struct {
+  int8_t *k, *v;
+  float *k_scales, *v_scales;
+  int n_slots, n_layers, max_seq, n_kv_heads, head_dim;
+} qasr_kv_int8;
+
+/* The rows of one call: n_seqs sequences whose rows are packed one after the
+ * other.  Sequence m has packed rows row_starts[m] .. row_starts[m+1]-1 (none
+ * when equal), which stand at rows positions[m] .. of cache slot slots[m]
+ * (slots NULL: slot m).  row_starts [n_seqs + 1], positions and slots are
+ * device arrays, read when the kernel runs, so a captured call follows their
+ * contents.  n_rows: rows of the packed buffers; those from
+ * row_starts[n_seqs] on are left as they are.  max_rows: at least the rows of
+ * the longest sequence (it sizes the launch).  A sequence whose entries do
+ * not fit (rows outside the packed buffers or the cache, more than max_rows
+ * rows, a slot outside the cache) is left out, its outputs unwritten, and sets
+ * *bad_flag (device, may be NULL; never cleared) to 1. */
+typedef struct {
+  const int32_t *row_starts, *positions, *slots;
+  int n_seqs, n_rows, max_rows;
+  int32_t *bad_flag;
+} qasr_kv_rows;
+
+/* qasr_kv_append for the INT8 cache: every head of the rows k_new, v_new
+ * [n_src, n_kv_heads * head_dim] is quantised by the rule of
+ * qasr_quantize_f32_to_int8 (absmax / 127, half away from zero) and written to
+ * its place in layer `layer`.  Packed row r takes source row src_rows[r]
+ * (device, [n_rows]), or source row r when src_rows is NULL (n_src >= n_rows):
+ * the accepted nodes of a drafted tree are written with one call.  A source
+ * row outside [0, n_src) is skipped and flagged.  A head holding NaN or an
+ * infinity is stored as scale NaN; one whose largest magnitude is below
+ * 2^-119 (127 / absmax overflows) as zeros.  No two sequences of a call may
+ * write the same cache row. */
+int qasr_kv_append_int8(const qasr_kv_int8 *cache, int layer, const qasr_kv_rows *rows, const float *k_new,
+                        const float *v_new, const int32_t *src_rows, int n_src, void *stream);
+
+/* The cache rows back as f32: k_out, v_out [n_rows, n_kv_heads * head_dim]
+ * (either may be NULL). */
+int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 *cache, int layer, const qasr_kv_rows *rows,
+                      void *stream);
+
+/* Attention of one or several tokens per sequence over the INT8 cache:
+ * sequence m's query rows q [n_rows, n_heads * head_dim] see its cache rows
+ * 0 .. positions[m]-1, and of the rows positions[m] + j, which hold the K/V of
+ * its own tokens (append them first), those that tree_mask allows: token t
+ * sees row j when bit j of tree_mask[row_starts[m] + t] is set (device,
+ * [n_rows]; sequences of at most 64 rows).  tree_mask NULL: j <= t, the
+ * causal rule of qasr_causal_attention; with one row per sequence this is a
+ * decode step, with many a prompt chunk.  out [n_rows, n_heads * head_dim] =
+ * softmax(scale * q k^T) v in f32; a row that sees nothing is zero.  n_heads
+ * a multiple of n_kv_heads, at most 64 query heads per kv head; q and out
+ * 16-byte aligned.  If a bounded device-side wait gives up, *bad_flag becomes
+ * -QASR_ERR_TIMEOUT. */
+int qasr_tree_attention_int8(float *out, const float *q, const qasr_kv_int8 *cache, int layer,
+                             const qasr_kv_rows *rows, const uint64_t *tree_mask, int n_heads, float scale,
+                             void *stream);
+
+/* Rules of qasr_logits_pick; every pointer is a device pointer and may be
+ * NULL (that rule is off).  Lists are packed: row m owns entries starts[m] ..
+ * starts[m+1]-1 (starts [M + 1]) of an array of n_... entries. */
+typedef struct {
+  const int32_t *history, *history_starts; /* tokens so far; a token may appear often */
+  int n_history;
+  const float *repetition, *presence, *frequency; /* [M]; need history */
+  const int32_t *bias_ids;  /* tokens with an additive bias; of several entries for one token the last counts */
+  const float *bias_values;
+  const int32_t *bias_starts;
+  int n_bias;
+  const uint32_t *allow_mask; /* [M, ceil(vocab / 32)]: bit t % 32 of word t / 32 set = token t allowed */
+  int32_t *bad_flag;          /* set to 1 by a list or token out of range (that list or entry is ignored) */
+} qasr_pick_rules;
+
+/* Token picks under rules, the step after qasr_final_norm_lmhead_argmax's
+ * logits_out.  For every row of logits [M, vocab], per token with value l
+ * that appears c times in the row's history:
+ *   c > 0:  l > 0 ? l / repetition : l * repetition,
+ *           minus (presence + frequency * c);
+ *   then plus its bias; a token that allow_mask does not allow becomes -inf.
+ * logits_out [M, vocab] (NULL, or logits itself, or disjoint from it) receives
+ * the values and ids [M] (may be NULL if logits_out is not) the first largest
+ * allowed one, NaN aside; -1 when there is none. */
+int qasr_logits_pick(int32_t *ids, float *logits_out, const float *logits, const qasr_pick_rules *rules, int M,
+                     int vocab, void *stream);
+
+/* ======================================================================
  * Decoder engine
  * ==================================================================== */
 

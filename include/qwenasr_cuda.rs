@@ -106,6 +106,32 @@ pub struct QasrStreamConfig {
     pub incremental: c_int,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct QasrKvInt8 {
+    pub k: *mut i8, pub v: *mut i8,
+    pub k_scales: *mut f32, pub v_scales: *mut f32,
+    pub n_slots: c_int, pub n_layers: c_int, pub max_seq: c_int, pub n_kv_heads: c_int, pub head_dim: c_int,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct QasrKvRows {
+    pub row_starts: *const i32, pub positions: *const i32, pub slots: *const i32,
+    pub n_seqs: c_int, pub n_rows: c_int, pub max_rows: c_int,
+    pub bad_flag: *mut i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct QasrPickRules {
+    pub history: *const i32, pub history_starts: *const i32, pub n_history: c_int,
+    pub repetition: *const f32, pub presence: *const f32, pub frequency: *const f32,
+    pub bias_ids: *const i32, pub bias_values: *const f32, pub bias_starts: *const i32, pub n_bias: c_int,
+    pub allow_mask: *const u32,
+    pub bad_flag: *mut i32,
+}
+
 #[link(name = "qwenasr_b200")]
 extern "C" {
     pub fn qasr_last_error() -> *const c_char;
@@ -143,6 +169,10 @@ extern "C" {
     pub fn qasr_int8_matvec_residual(x: *mut f32, a: *const f32, w: *const i8, scales: *const f32, M: c_int, in_dim: c_int, out_dim: c_int, stream: *mut c_void) -> c_int;
     pub fn qasr_final_norm_lmhead_argmax(ids_out: *mut i32, logits_out: *mut f32, x: *const f32, norm_w: *const f32, w: *const i8, scales: *const f32, M: c_int, hidden: c_int, vocab: c_int, eps: f32, stream: *mut c_void) -> c_int;
     pub fn qasr_final_norm_lmhead_argmax_noalloc(ids_out: *mut i32, logits_out: *mut f32, x: *const f32, norm_w: *const f32, w: *const i8, scales: *const f32, M: c_int, hidden: c_int, vocab: c_int, eps: f32, stream: *mut c_void) -> c_int;
+    pub fn qasr_kv_append_int8(cache: *const QasrKvInt8, layer: c_int, rows: *const QasrKvRows, k_new: *const f32, v_new: *const f32, src_rows: *const i32, n_src: c_int, stream: *mut c_void) -> c_int;
+    pub fn qasr_kv_read_int8(k_out: *mut f32, v_out: *mut f32, cache: *const QasrKvInt8, layer: c_int, rows: *const QasrKvRows, stream: *mut c_void) -> c_int;
+    pub fn qasr_tree_attention_int8(out: *mut f32, q: *const f32, cache: *const QasrKvInt8, layer: c_int, rows: *const QasrKvRows, tree_mask: *const u64, n_heads: c_int, scale: f32, stream: *mut c_void) -> c_int;
+    pub fn qasr_logits_pick(ids: *mut i32, logits_out: *mut f32, logits: *const f32, rules: *const QasrPickRules, m: c_int, vocab: c_int, stream: *mut c_void) -> c_int;
     pub fn qasr_decoder_create(cfg: *const QasrDecoderConfig, device: c_int) -> *mut QasrDecoder;
     pub fn qasr_decoder_free(dec: *mut QasrDecoder);
     pub fn qasr_decoder_set_layer(dec: *mut QasrDecoder, layer: c_int, w: *const QasrDecLayerWeights) -> c_int;

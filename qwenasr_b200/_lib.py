@@ -39,6 +39,23 @@ class DecLayerWeights(C.Structure):
         "q_norm", "k_norm", "input_norm", "post_attn_norm")]
 
 
+class KvInt8(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scales", "v_scales")] + \
+               [(n, C.c_int) for n in ("n_slots", "n_layers", "max_seq", "n_kv_heads", "head_dim")]
+
+
+class KvRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("row_starts", "positions", "slots")] + \
+               [(n, C.c_int) for n in ("n_seqs", "n_rows", "max_rows")] + [("bad_flag", C.c_void_p)]
+
+
+class PickRules(C.Structure):
+    _fields_ = [("history", C.c_void_p), ("history_starts", C.c_void_p), ("n_history", C.c_int),
+                ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p), ("bias_starts", C.c_void_p),
+                ("n_bias", C.c_int), ("allow_mask", C.c_void_p), ("bad_flag", C.c_void_p)]
+
+
 P = C.c_void_p
 I = C.c_int
 I64 = C.c_int64
@@ -81,6 +98,10 @@ _SIGS = {
     "qasr_int8_matvec_residual": (I, [P, P, P, P, I, I, I, P]),
     "qasr_final_norm_lmhead_argmax": (I, [P, P, P, P, P, P, I, I, I, F, P]),
     "qasr_final_norm_lmhead_argmax_noalloc": (I, [P, P, P, P, P, P, I, I, I, F, P]),
+    "qasr_kv_append_int8": (I, [C.POINTER(KvInt8), I, C.POINTER(KvRows), P, P, P, I, P]),
+    "qasr_kv_read_int8": (I, [P, P, C.POINTER(KvInt8), I, C.POINTER(KvRows), P]),
+    "qasr_tree_attention_int8": (I, [P, P, C.POINTER(KvInt8), I, C.POINTER(KvRows), P, I, F, P]),
+    "qasr_logits_pick": (I, [P, P, P, C.POINTER(PickRules), I, I, P]),
     "qasr_decoder_create": (P, [C.POINTER(DecoderConfig), I]),
     "qasr_decoder_free": (None, [P]),
     "qasr_decoder_set_layer": (I, [P, I, C.POINTER(DecLayerWeights)]),

@@ -21,6 +21,7 @@ __all__ = [
     "kv_append", "sinusoidal_pe", "gelu", "gelu_erf", "silu", "swiglu_multiply", "add_inplace",
     "linear_nobias_int8", "linear_int8", "causal_attention", "quantize_f32_to_int8", "embed_gather",
     "pre_attn_block", "ln_pe", "ln_pe_gelu_erf", "int8_norm_gateup_swiglu", "int8_matvec_residual", "final_norm_lmhead_argmax",
+    "kv_append_int8", "kv_read_int8", "tree_attention_int8", "logits_pick",
 ]
 
 
@@ -262,3 +263,85 @@ def final_norm_lmhead_argmax(ids_out, logits_out, x, norm_w, w, scales, M, hidde
               _ptr(logits_out, f32, "logits_out", M * vocab), _ptr(x, f32, "x", M * hidden),
               _ptr(norm_w, f32, "norm_w", hidden), _ptr(w, i8, "w", vocab * hidden), _ptr(scales, f32, "scales", vocab),
               M, hidden, vocab, C.c_float(eps), _stream())
+
+
+# ---------------------------------------------------------------- serving --
+def _need(t, dtype, device, name, numel):
+    """_ptr for an operand that must also lie on `device`."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise ValueError(f"{name} must be a tensor on {device}")
+    return _ptr(t, dtype, name, numel)
+
+
+def _on(device, name, *args):
+    """Call an entry on `device`, on that device's current stream (the last argument)."""
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _stream())
+
+
+def _kv_args(cache, rows):
+    if rows.device != cache.device:
+        raise ValueError(f"rows are on {rows.device}, the cache on {cache.device}")
+    return cache.device, rows.n_rows
+
+
+def kv_append_int8(cache, layer, rows, k_new, v_new, src_rows=None):
+    """Quantise rows k_new, v_new [n, n_kv_heads * head_dim] into layer `layer`
+    of a KvCacheInt8 at the places of `rows` (KvRows); packed row r takes source
+    row src_rows[r] (int32) or r.  The f32 form is kv_append."""
+    dev, n = _kv_args(cache, rows)
+    need = 0 if src_rows is not None else n * cache.kv_dim
+    k, v = _need(k_new, f32, dev, "k_new", need), _need(v_new, f32, dev, "v_new", need)
+    _on(dev, "qasr_kv_append_int8", C.byref(cache.c), layer, C.byref(rows.c), k, v,
+        _need(src_rows, i32, dev, "src_rows", n), min(k_new.numel(), v_new.numel()) // cache.kv_dim)
+
+
+def kv_read_int8(k_out, v_out, cache, layer, rows):
+    """The cache rows of `rows` as f32 into k_out, v_out [n_rows, n_kv_heads * head_dim]; either may be None."""
+    dev, n = _kv_args(cache, rows)
+    _on(dev, "qasr_kv_read_int8", _need(k_out, f32, dev, "k_out", n * cache.kv_dim),
+        _need(v_out, f32, dev, "v_out", n * cache.kv_dim), C.byref(cache.c), layer, C.byref(rows.c))
+
+
+def tree_attention_int8(out, q, cache, layer, rows, n_heads, scale, tree_mask=None):
+    """Attention of the query rows q [n_rows, n_heads * head_dim] over their
+    sequences' cache rows: the past, and of their own rows those the int64
+    tree_mask [n_rows] allows (bit j: row j of the sequence), or the causal ones
+    when it is None.  The rows' own K/V are appended first."""
+    dev, n = _kv_args(cache, rows)
+    size = n * n_heads * cache.head_dim
+    _on(dev, "qasr_tree_attention_int8", _need(out, f32, dev, "out", size), _need(q, f32, dev, "q", size),
+        C.byref(cache.c), layer, C.byref(rows.c), _need(tree_mask, torch.int64, dev, "tree_mask", n), n_heads,
+        C.c_float(scale))
+
+
+def logits_pick(ids_out, logits_out, logits, M, vocab, history=None, history_starts=None, repetition=None,
+                presence=None, frequency=None, bias_ids=None, bias_values=None, bias_starts=None, allow_mask=None,
+                bad_flag=None):
+    """Penalties of repeated tokens, biases and the mask of allowed tokens on
+    logits [M, vocab], then the first-max pick (qasr_logits_pick).  ids_out or
+    logits_out may be None; logits_out may be logits.  Lists are packed with
+    starts [M + 1]; allow_mask is int32 [M, ceil(vocab / 32)], bit set = allowed."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor")
+    dev = logits.device
+
+    def opt(t, dtype, name, numel):
+        return None if t is None else _need(t, dtype, dev, name, numel).value
+
+    n_bias = 0 if bias_ids is None else bias_ids.numel()
+    r = _lib.PickRules(opt(history, i32, "history", 0), opt(history_starts, i32, "history_starts", M + 1),
+                       0 if history is None else history.numel(), opt(repetition, f32, "repetition", M),
+                       opt(presence, f32, "presence", M), opt(frequency, f32, "frequency", M),
+                       opt(bias_ids, i32, "bias_ids", 0), opt(bias_values, f32, "bias_values", n_bias),
+                       opt(bias_starts, i32, "bias_starts", M + 1), n_bias,
+                       opt(allow_mask, i32, "allow_mask", M * ((vocab + 31) // 32)),
+                       opt(bad_flag, i32, "bad_flag", 1))
+    _on(dev, "qasr_logits_pick", _need(ids_out, i32, dev, "ids_out", M),
+        _need(logits_out, f32, dev, "logits_out", M * vocab), _need(logits, f32, dev, "logits", M * vocab), C.byref(r),
+        M, vocab)
