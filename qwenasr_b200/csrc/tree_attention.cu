@@ -5,11 +5,117 @@
 //   S_tj = scale * sum_d q_td kc_jd * ks_j
 //   out_t = sum_j e^(S_tj - max_j S_tj) * vs_j * vc_j / sum_j e^(S_tj - max_j S_tj)
 // over the rows j that t sees; nothing visible gives zero.
+//
+// Both products run on the tensor cores (tcgen05, kind::i8) on the codes as
+// they lie in the cache, exactly in 32-bit integers:
+//  * a query row is scaled by a power of two 2^(22-E) (2^E bounds its largest
+//    magnitude), rounded to an integer and split into three signed base-256
+//    digits, as in the INT8 projections.  S^T [keys x 3 digit planes of the
+//    rows] = K codes [128 keys x 128] * digits^T; the rounding of q is half a
+//    step of 2^-22 of the row's largest magnitude.
+//  * a weight e^(S - tile maximum) * vs_j / (tile's largest vs) lies in [0, 1];
+//    2^23 - 1 of it, rounded, are three unsigned digits (the low bytes of the
+//    float 2^23 + that), off by at most 2^-24 of the largest weight of the
+//    tile, below the f32 rounding of a sum over it.  O^T [128 values x digit
+//    planes] = V codes^T * digits, with V read as it lies (M-major) and the
+//    digits written by the thread that owns the key (N-major): nothing is
+//    transposed or converted on the way.
+// Digit sums are recombined in f32 (one rounding below the value's own) and
+// accumulated over the tiles in f32 with the usual running maximum and sum.
+//
+// Keys sit on the M side (128 TMEM lanes, one thread each), rows on the N
+// side: one query row then costs 16 columns instead of a 128-row tile, which
+// is what a decode step needs, and the work per key grows with the rows that
+// are there.  Two kv heads of 64 values share one 128-wide tile: the digits of
+// a row are zero in the other head's half, and its half of O is dropped.
+//
+// A cluster of C CTAs shares one (sequence, kv head, block of NR rows): each
+// takes a run of 128-key tiles, the partial states are pushed to the CTA that
+// finishes a row over distributed shared memory, so a call needs no
+// workspace, no atomics and no second launch.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
 #include "kv_int8.cuh"
+#include "tcgen05.cuh"
+#include "tma.cuh"
+#include "umma.cuh"
 
 namespace qasr {
 
+// Three planes of 4 consecutive columns of this warp's 32 TMEM lanes, at
+// columns 0, stride and 2 * stride of taddr.
+QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%12];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%4, %5, %6, %7}, [%13];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%8, %9, %10, %11}, [%14];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(d[0][0]), "=r"(d[0][1]), "=r"(d[0][2]), "=r"(d[0][3]), "=r"(d[1][0]), "=r"(d[1][1]),
+        "=r"(d[1][2]), "=r"(d[1][3]), "=r"(d[2][0]), "=r"(d[2][1]), "=r"(d[2][2]), "=r"(d[2][3])
+      : "r"(taddr), "r"(taddr + stride), "r"(taddr + 2 * stride)
+      : "memory");
+}
+
+// Three planes of 8 consecutive columns of this warp's 32 TMEM lanes, at
+// columns 0, stride and 2 * stride of taddr.
+QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%24];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%25];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16, %17, %18, %19, %20, %21, %22, %23}, [%26];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(d[0][0]), "=r"(d[0][1]), "=r"(d[0][2]), "=r"(d[0][3]), "=r"(d[0][4]), "=r"(d[0][5]),
+        "=r"(d[0][6]), "=r"(d[0][7]), "=r"(d[1][0]), "=r"(d[1][1]), "=r"(d[1][2]), "=r"(d[1][3]),
+        "=r"(d[1][4]), "=r"(d[1][5]), "=r"(d[1][6]), "=r"(d[1][7]), "=r"(d[2][0]), "=r"(d[2][1]),
+        "=r"(d[2][2]), "=r"(d[2][3]), "=r"(d[2][4]), "=r"(d[2][5]), "=r"(d[2][6]), "=r"(d[2][7])
+      : "r"(taddr), "r"(taddr + stride), "r"(taddr + 2 * stride)
+      : "memory");
+}
+
+// Three planes of 16 consecutive columns of this warp's 32 TMEM lanes, at
+// columns 0, stride and 2 * stride of taddr.
+QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%48];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%49];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47}, [%50];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(d[0][0]), "=r"(d[0][1]), "=r"(d[0][2]), "=r"(d[0][3]), "=r"(d[0][4]), "=r"(d[0][5]),
+        "=r"(d[0][6]), "=r"(d[0][7]), "=r"(d[0][8]), "=r"(d[0][9]), "=r"(d[0][10]), "=r"(d[0][11]),
+        "=r"(d[0][12]), "=r"(d[0][13]), "=r"(d[0][14]), "=r"(d[0][15]), "=r"(d[1][0]), "=r"(d[1][1]),
+        "=r"(d[1][2]), "=r"(d[1][3]), "=r"(d[1][4]), "=r"(d[1][5]), "=r"(d[1][6]), "=r"(d[1][7]),
+        "=r"(d[1][8]), "=r"(d[1][9]), "=r"(d[1][10]), "=r"(d[1][11]), "=r"(d[1][12]), "=r"(d[1][13]),
+        "=r"(d[1][14]), "=r"(d[1][15]), "=r"(d[2][0]), "=r"(d[2][1]), "=r"(d[2][2]), "=r"(d[2][3]),
+        "=r"(d[2][4]), "=r"(d[2][5]), "=r"(d[2][6]), "=r"(d[2][7]), "=r"(d[2][8]), "=r"(d[2][9]),
+        "=r"(d[2][10]), "=r"(d[2][11]), "=r"(d[2][12]), "=r"(d[2][13]), "=r"(d[2][14]), "=r"(d[2][15])
+      : "r"(taddr), "r"(taddr + stride), "r"(taddr + 2 * stride)
+      : "memory");
+}
+
+constexpr int kTaKeys = 128;             // keys of a tile: TMEM lanes of S^T
+constexpr int kTaTile = kTaKeys * 128;   // bytes of a K (or V) tile
+constexpr int kTaThreads = 192;          // 4 softmax warps, the MMA warp, the TMA warp
+constexpr int kTaMaxCluster = 16;
+constexpr float kTaOne = 8388607.0f;     // a weight of 1
+constexpr float kTaMagic = 8388608.0f;   // 2^23: its low three bytes are zero
+
+// Rows of a block: NR query rows, their digit planes side by side (plane d at
+// column d * NR), N columns for the tensor cores (a multiple of 16).
+template <int NR>
+struct TaShape {
+  static_assert(NR == 4 || NR == 8 || NR == 16 || NR == 32, "rows of a block");
+  static constexpr int kN = NR == 4 ? 16 : NR == 8 ? 32 : 3 * NR;
+  static constexpr int kTmem = NR == 32 ? 256 : NR == 16 ? 128 : NR == 8 ? 64 : 32;  // S and O, a power of two
+  static constexpr int kStages = NR <= 8 ? 3 : 2;  // K and V tiles in flight
+  static constexpr int kChunk = NR < 16 ? NR : 16;  // rows per TMEM load
+  static constexpr int kQBytes = kN * 128, kPBytes = kN * 128;
+};
+
 struct TreeAttnParams {
+  CUtensorMap tm_k, tm_v;  // codes as [cache rows, kv_dim], box 128 rows x 128 bytes, 128-byte swizzle
   float *out;
   const float *q;
   qasr_kv_int8 c;
@@ -19,68 +125,502 @@ struct TreeAttnParams {
   float scale;
 };
 
-// Cache rows below the sequence's first token are past; row pos + j is token
-// j's, visible by the mask or, without one, to the tokens from j on.
-QASR_DEV bool tree_visible(int place, int t, int n, bool tree, uint64_t mask) {
-  if (place < 0) return true;
-  if (place >= n) return false;
-  return tree ? (mask >> place & 1) != 0 : place <= t;
+template <int NR>
+struct TaSmem {
+  alignas(1024) unsigned char ring[TaShape<NR>::kStages][2][kTaTile];  // K, V
+  alignas(1024) unsigned char q[TaShape<NR>::kQBytes];  // digits, K-major, 128-byte swizzle
+  alignas(1024) unsigned char p[TaShape<NR>::kPBytes];  // digits, N-major, no swizzle
+  // partial states pushed by the cluster: entry r / C * C + c is CTA c's of row r, one of the rows r % C = rank
+  static constexpr int kRecv = NR < kTaMaxCluster ? kTaMaxCluster : NR;
+  float recv[kRecv][128], recv_m[kRecv], recv_l[kRecv];
+  float4 rowc[2][4][NR];  // per tile (two in flight) and warp: tile maximum, factors of the new and old sums, of O
+  float wmax[2][4][NR];   // per tile and warp: row maxima
+  float wvs[2][4][2];     // ... and largest value scales
+  float qf[NR];           // 2^(E-22) * scale * log2(e)
+  float lsum[4][NR];
+  uint64_t mask[NR];
+  int tok[NR];            // the row's token, -1 for none
+  uint64_t full_k[3], full_v[3], empty[3], sfull, sfree, pready, ofull, qready, done;
+  uint32_t tmem;
+  int abort;
+};
+
+// Descriptor of the digits P: N-major without swizzle, 16 columns x 8 keys per
+// 128-byte core matrix, the next 8 keys 128 bytes on, the next 16 columns
+// 2048 bytes on (128 keys).
+QASR_DEV uint64_t ta_desc_p(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(2048 >> 4) << 32 |
+         (uint64_t)1 << 46;
 }
 
-// One warp per (sequence, query head, token): 32 keys a round, one per lane
-// for the scores, HD / 32 output values per lane.
-template <int HD>
-__global__ void __launch_bounds__(128) tree_attention_kernel(const TreeAttnParams p) {
-  __shared__ __align__(16) float sq[4][HD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m = blockIdx.z, h = blockIdx.y, t = blockIdx.x * 4 + warp;
-  if (blockIdx.x == 0 && h == 0 && m == 0 && warp == 0) kv_flag_bad(p.r, p.c, lane);
-  const KvSeq s = kv_seq(p.r, p.c, m);
-  if (t >= s.n) return;
-  const int kvh = h / (p.n_heads / p.c.n_kv_heads);
-  const size_t row = s.row0 + t, kv_dim = (size_t)p.c.n_kv_heads * HD;
-  const float *q = p.q + (row * p.n_heads + h) * HD;
-  for (int d = lane; d < HD; d += 32) sq[warp][d] = q[d];
-  __syncwarp();
-  const uint64_t mask = p.tree_mask ? p.tree_mask[row] : 0;
-  const size_t base = kv_row(p.c, s.slot, p.layer, 0);
-  const int len = s.pos + s.n;
-  float mx = -INFINITY, l = 0.0f, o[HD / 32] = {};
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int j = j0 + lane;
-    float sc = -INFINITY, vs = 0.0f;
-    if (j < len && tree_visible(j - s.pos, t, s.n, p.tree_mask != nullptr, mask)) {
-      const uint32_t *k = reinterpret_cast<const uint32_t *>(p.c.k + (base + j) * kv_dim + (size_t)kvh * HD);
-      float a = 0.0f;
-      for (int d = 0; d < HD / 4; ++d) {
-        float f[4];
-        i8x4_to_f32(k[d], f);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a = fmaf(sq[warp][4 * d + e], f[e], a);
-      }
-      sc = a * p.c.k_scales[(base + j) * p.c.n_kv_heads + kvh] * p.scale;
-      vs = p.c.v_scales[(base + j) * p.c.n_kv_heads + kvh];
-    }
-    const bool nan = __any_sync(0xffffffffu, sc != sc);
-    const float mn = nan ? __uint_as_float(0x7fc00000u) : fmaxf(mx, warp_max(sc));
-    if (mn == -INFINITY) continue;
-    const float corr = mx == -INFINITY ? 0.0f : expf(mx - mn);
-    const float pj = sc == -INFINITY ? 0.0f : expf(sc - mn);
-    mx = mn;
-    l = l * corr + warp_sum(pj);
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) o[e] *= corr;
-    const float w = sc == -INFINITY ? 0.0f : pj * vs;
-    for (int i = 0; i < min(32, len - j0); ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const int8_t *v = p.c.v + (base + j0 + i) * kv_dim + (size_t)kvh * HD;
-#pragma unroll
-      for (int e = 0; e < HD / 32; ++e) o[e] = fmaf(wi, (float)v[lane + 32 * e], o[e]);
+// kind::i8, S32 sums; A signed, B signed (S) or unsigned (O), both K-major (S)
+// or both M/N-major (O).
+constexpr uint32_t ta_idesc_s(int N) { return umma_idesc_s8(128, N); }
+constexpr uint32_t ta_idesc_o(int N) {
+  return (2u << 4) | (1u << 7) | (1u << 15) | (1u << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+QASR_DEV float ta_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+QASR_DEV float ta_warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+QASR_DEV void ta_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+QASR_DEV void ta_store_remote(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// Bounded wait that also gives up once another role has.
+template <int NR>
+QASR_DEV bool ta_wait(TaSmem<NR> &sm, uint64_t *bar, unsigned parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*reinterpret_cast<volatile int *>(&sm.abort)) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      atomicExch(&sm.abort, 1);
+      return false;
     }
   }
-  float *out = p.out + (row * p.n_heads + h) * HD;
+  return true;
+}
+
+// Digits of four q values at bytes b .. b+3 of digit row n = r, r + NR, r + 2 NR.
+template <int NR>
+QASR_DEV void ta_put_digits(unsigned char *q, int r, int b, float4 v, float qm) {
+  int X[4] = {__float_as_int(fmaf(v.x, qm, 12582912.0f)) - 0x4B400000,
+              __float_as_int(fmaf(v.y, qm, 12582912.0f)) - 0x4B400000,
+              __float_as_int(fmaf(v.z, qm, 12582912.0f)) - 0x4B400000,
+              __float_as_int(fmaf(v.w, qm, 12582912.0f)) - 0x4B400000};
 #pragma unroll
-  for (int e = 0; e < HD / 32; ++e) out[lane + 32 * e] = l == 0.0f ? 0.0f : o[e] / l;
+  for (int d = 2; d >= 0; --d) {  // balanced: -128 .. 127, the carry goes up
+    const uint32_t w =
+        __byte_perm(__byte_perm(X[0], X[1], 0x0040), __byte_perm(X[2], X[3], 0x0040), 0x5410);
+    const int n = d * NR + r;
+    *reinterpret_cast<uint32_t *>(q + n * 128 + (((b >> 4) ^ (n & 7)) << 4) + (b & 15)) = w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) X[i] = (X[i] + 128) >> 8;
+  }
+}
+
+// HD: head_dim; HPB = 128 / HD kv heads share a tile.  Grid: (C, head blocks x
+// row blocks, sequences), clusters of C along x.
+template <int HD, int NR>
+__global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
+  using Sh = TaShape<NR>;
+  constexpr int HPB = 128 / HD, N = Sh::kN, ST = Sh::kStages, CH = Sh::kChunk;
+  extern __shared__ unsigned char smem_raw[];
+  TaSmem<NR> &sm = *reinterpret_cast<TaSmem<NR> *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = gridDim.x, rank = blockIdx.x, m = blockIdx.z;
+  const int G = p.n_heads / p.c.n_kv_heads, W = HPB * G;  // query rows of one token in a block
+  const int hblocks = (p.c.n_kv_heads + HPB - 1) / HPB, hb = blockIdx.y % hblocks, rb = blockIdx.y / hblocks;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && m == 0 && warp == 5) kv_flag_bad(p.r, p.c, lane);
+  const KvSeq s = kv_seq(p.r, p.c, m);
+  const int v0 = rb * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
+  if (rows <= 0) return;                                 // the whole cluster
+  const bool tree = p.tree_mask != nullptr;
+  const int len = s.pos + (tree ? s.n : (v0 + rows - 1) / W + 1);  // keys any row may see
+  const int tiles = (len + kTaKeys - 1) / kTaKeys;
+  const int i0 = (int)((long)tiles * rank / C), n = (int)((long)tiles * (rank + 1) / C) - i0;
+
+  if (C > 1) cluster_arrive_all();  // waited for before the first remote store: every CTA has started
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&sm.full_k[i], 1);
+      mbar_init(&sm.full_v[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    mbar_init(&sm.sfull, 1);
+    mbar_init(&sm.sfree, 4);
+    mbar_init(&sm.pready, 4);
+    mbar_init(&sm.ofull, 1);
+    mbar_init(&sm.qready, 4);
+    mbar_init(&sm.done, 1);
+    sm.abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 4) tmem_alloc(&sm.tmem, Sh::kTmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem, tmem_o = tmem + N;
+
+  float acc[NR], l[NR], m_run = -INFINITY;  // thread = value column (acc), key (l); lane = row (m_run)
+#pragma unroll
+  for (int r = 0; r < NR; ++r) acc[r] = l[r] = 0.0f;
+
+  if (warp == 5) {
+    // ---------------------------------------------------------------- TMA
+    if (lane == 0 && n > 0) {
+      const int row = (int)kv_row(p.c, s.slot, p.layer, 0);
+      int i = 0;
+      for (; i < n; ++i) {
+        const int st = i % ST;
+        if (i >= ST && !ta_wait(sm, &sm.empty[st], (unsigned)((i / ST - 1) & 1))) break;
+        const int y = row + (i0 + i) * kTaKeys;
+        mbar_arrive_expect_tx(&sm.full_k[st], kTaTile);
+        tma_load_2d_u8(sm.ring[st][0], &p.tm_k, hb * 128, y, &sm.full_k[st]);
+        mbar_arrive_expect_tx(&sm.full_v[st], kTaTile);
+        tma_load_2d_u8(sm.ring[st][1], &p.tm_v, hb * 128, y, &sm.full_v[st]);
+      }
+      // copies that nobody waited for (after a timeout) land before the CTA leaves
+      for (int k = max(0, i - ST); k < i; ++k) {
+        mbar_wait(&sm.full_k[k % ST], (unsigned)((k / ST) & 1));
+        mbar_wait(&sm.full_v[k % ST], (unsigned)((k / ST) & 1));
+      }
+    }
+  } else if (warp == 4) {
+    // ---------------------------------------------------------------- MMA
+    if (lane == 0 && n > 0) {
+      const uint32_t qa = smem_u32(sm.q), pa = smem_u32(sm.p);
+      auto scores = [&](int i) {
+        const int st = i % ST;
+        if (!ta_wait(sm, &sm.full_k[st], (unsigned)((i / ST) & 1))) return false;
+        tc_fence_after();
+        const uint32_t ka = smem_u32(sm.ring[st][0]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_s8(tmem, umma_desc_sw128(ka + 32 * k), umma_desc_sw128(qa + 32 * k), ta_idesc_s(N), k > 0);
+        umma_commit(&sm.sfull);
+        return true;
+      };
+      bool ok = ta_wait(sm, &sm.qready, 0) && scores(0);
+      for (int i = 0; ok && i < n; ++i) {
+        const int st = i % ST;
+        if (i + 1 < n) ok = ta_wait(sm, &sm.sfree, (unsigned)(i & 1)) && scores(i + 1);
+        ok = ok && ta_wait(sm, &sm.full_v[st], (unsigned)((i / ST) & 1)) && ta_wait(sm, &sm.pready, (unsigned)(i & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = smem_u32(sm.ring[st][1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // 32 keys a step: four 8-key groups of 1024 (V) and 128 (P) bytes
+          umma_s8(tmem_o, umma_desc_sw128(va + 4096 * k), ta_desc_p(pa + 512 * k), ta_idesc_o(N), k > 0);
+        umma_commit(&sm.empty[st]);
+        umma_commit(&sm.ofull);
+      }
+      if (!ok) {  // after a timeout: the products in flight end before TMEM is freed
+        umma_commit(&sm.done);
+        mbar_wait(&sm.done, 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    for (int r = warp; r < NR; r += 4) {
+      const int v = v0 + r, t = r < rows ? v / W : -1, h = v % W, b = 4 * lane - h / G * HD;  // b: value of the head
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (t >= 0 && b >= 0 && b < HD && hb * W + h < p.n_heads)
+        x = *reinterpret_cast<const float4 *>(p.q + ((size_t)(s.row0 + t) * p.n_heads + hb * W + h) * HD + b);
+      constexpr uint32_t kAbs = 0x7fffffffu;
+      const uint32_t top = __reduce_max_sync(
+          0xffffffffu, max(max(__float_as_uint(x.x) & kAbs, __float_as_uint(x.y) & kAbs),
+                           max(__float_as_uint(x.z) & kAbs, __float_as_uint(x.w) & kAbs)));
+      // 2^E above the largest magnitude; below 2^-100 the scores are as good as zero.  NaN or an infinity
+      // (all exponent bits) makes the row's factor, and so its scores, NaN.
+      const int e = max((int)(top >> 23) - 126, -100);
+      ta_put_digits<NR>(sm.q, r, 4 * lane, x, __int_as_float((127 + 22 - e) << 23));
+      if (lane == 0) {
+        const float f = __fmul_rn(__int_as_float((127 + e - 22) << 23), __fmul_rn(p.scale, 1.44269504088896341f));
+        sm.qf[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : f;
+        sm.tok[r] = t;
+        sm.mask[r] = t >= 0 && tree ? p.tree_mask[s.row0 + t] : 0;
+      }
+    }
+    for (int b = 3 * NR * 128 + 4 * tid; b < Sh::kQBytes; b += 512) *reinterpret_cast<uint32_t *>(sm.q + b) = 0;
+    fence_proxy_async();
+    named_bar(1, 128);
+    if (lane == 0) ta_arrive(&sm.qready);
+    const uint32_t my_s = tmem + ((uint32_t)warp << 21), my_o = tmem_o + ((uint32_t)warp << 21);
+    const size_t srow = kv_row(p.c, s.slot, p.layer, 0);
+    float nks[HPB], nvs[HPB];  // scales of this thread's key of the next tile
+    auto load_scales = [&](int i) {
+      const int j = (i0 + i) * kTaKeys + tid;
+#pragma unroll
+      for (int u = 0; u < HPB; ++u) {
+        const bool in = i < n && j < len && hb * HPB + u < p.c.n_kv_heads;
+        const size_t at = (srow + j) * p.c.n_kv_heads + hb * HPB + u;
+        nks[u] = in ? __ldg(p.c.k_scales + at) : 0.0f;
+        nvs[u] = in ? __ldg(p.c.v_scales + at) : 0.0f;
+      }
+    };
+    // Second kv head of the pair for this row (HPB = 2).
+    auto second = [&](int r) { return HPB == 2 && (v0 + r) % W >= G; };
+    uint32_t hi = 0;  // bit r: row r is of the pair's second head
+    if constexpr (HPB == 2) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) hi |= second(r) ? 1u << r : 0u;
+    }
+    // acc = acc * old + O * coef for the tile whose constants are in rowc[b]
+    auto fold = [&](int b) {
+#pragma unroll
+      for (int c0 = 0; c0 < NR; c0 += CH) {
+        uint32_t d[3][CH];
+        tmem_ld_planes(my_o + c0, NR, d);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const float4 c = sm.rowc[b][warp][c0 + i];
+          const float o = fmaf((float)(int)d[2][i], 65536.0f, (float)((int)d[1][i] * 256 + (int)d[0][i]));
+          acc[c0 + i] = fmaf(acc[c0 + i], c.z, __fmul_rn(o, c.w));
+        }
+      }
+    };
+    // After a timeout (sm.abort) every wait returns at once and the loop runs on: the four warps must meet at
+    // the same number of barriers.  The results are thrown away.
+    load_scales(0);
+    for (int i = 0; i < n; ++i) {
+      const int buf = i & 1, j = (i0 + i) * kTaKeys + tid;
+      float ks[HPB], vs[HPB];
+#pragma unroll
+      for (int u = 0; u < HPB; ++u) ks[u] = nks[u], vs[u] = nvs[u];
+      load_scales(i + 1);
+      ta_wait(sm, &sm.sfull, (unsigned)(i & 1));
+      __syncwarp();
+      tc_fence_after();
+      float x[NR];  // scores in units of log 2
+#pragma unroll
+      for (int c0 = 0; c0 < NR; c0 += CH) {
+        uint32_t d[3][CH];
+        tmem_ld_planes(my_s + c0, NR, d);
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+          const int r = c0 + e;
+          const float k = HPB == 2 && (hi >> r & 1) ? ks[HPB - 1] : ks[0];
+          const float sum = fmaf((float)(int)d[0][e], 65536.0f, (float)((int)d[1][e] * 256 + (int)d[2][e]));
+          x[r] = __fmul_rn(sum, __fmul_rn(sm.qf[r], k));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ta_arrive(&sm.sfree);
+      const int place = j - s.pos;  // >= 0: the row of one of the sequence's own tokens
+      if ((i0 + i + 1) * kTaKeys > s.pos) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const bool see = place < 0 || (place < s.n && (tree ? sm.mask[r] >> (place & 63) & 1 : place <= sm.tok[r]));
+          if (!see) x[r] = -INFINITY;
+        }
+      }
+      // a value scale that is no finite number >= 0 counts as NaN, for the rows that see it
+      bool odd[HPB];
+#pragma unroll
+      for (int u = 0; u < HPB; ++u) {
+        odd[u] = !(vs[u] >= 0.0f && vs[u] < INFINITY);
+        if (odd[u]) vs[u] = 0.0f;
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vs[u])));
+        if (lane == 0) sm.wvs[buf][warp][u] = top;
+      }
+      float mine = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float t = ta_warp_max(x[r]);
+        if (lane == r) mine = t;
+      }
+      if (lane < NR) sm.wmax[buf][warp][lane] = mine;
+      named_bar(1, 128);
+      float vmax[HPB];
+#pragma unroll
+      for (int u = 0; u < HPB; ++u) {
+        vmax[u] = fmaxf(fmaxf(sm.wvs[buf][0][u], sm.wvs[buf][1][u]), fmaxf(sm.wvs[buf][2][u], sm.wvs[buf][3][u]));
+        vs[u] = vmax[u] > 0.0f ? __fdiv_rn(vs[u], vmax[u]) : 0.0f;
+      }
+      if (lane < NR) {
+        const float t = fmaxf(fmaxf(sm.wmax[buf][0][lane], sm.wmax[buf][1][lane]),
+                              fmaxf(sm.wmax[buf][2][lane], sm.wmax[buf][3][lane]));
+        const float top = fmaxf(m_run, t), base = top == -INFINITY ? 0.0f : top;
+        const float f = t == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(t, base));
+        const float old = m_run == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(m_run, base));
+        const float vm = HPB == 2 && (hi >> lane & 1) ? vmax[HPB - 1] : vmax[0];
+        sm.rowc[buf][warp][lane] =
+            make_float4(t == -INFINITY ? 0.0f : t, f, old, __fmul_rn(f, __fmul_rn(vm, 1.0f / kTaOne)));
+        m_run = top;
+      }
+      __syncwarp();
+      bool any_odd = odd[0];
+      if constexpr (HPB == 2) any_odd |= odd[HPB - 1];
+      if (__any_sync(0xffffffffu, any_odd)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          if (x[r] != -INFINITY && (HPB == 2 && (hi >> r & 1) ? odd[HPB - 1] : odd[0])) l[r] = __uint_as_float(0x7fc00000u);
+      }
+      if (i > 0) {  // the previous tile's O; its digits in sm.p are free after it
+        ta_wait(sm, &sm.ofull, (unsigned)((i - 1) & 1));
+        __syncwarp();
+        tc_fence_after();
+        fold(buf ^ 1);
+      }
+      uint32_t w[3 * NR / 4 + (NR == 4 ? 1 : NR == 8 ? 2 : 0)];
+      w[3 * NR / 4 - 1 + (NR == 4 ? 1 : NR == 8 ? 2 : 0)] = 0;  // unused columns
+      if constexpr (NR == 8) w[6] = 0;
+#pragma unroll
+      for (int r0 = 0; r0 < NR; r0 += 4) {
+        uint32_t f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = r0 + e;
+          const float4 c = sm.rowc[buf][warp][r];
+          const float pr = ta_ex2(__fsub_rn(x[r], c.x));
+          l[r] = fmaf(l[r], c.z, __fmul_rn(pr, c.y));
+          const float v = HPB == 2 && (hi >> r & 1) ? vs[HPB - 1] : vs[0];
+          f[e] = __float_as_uint(fmaf(__fmul_rn(pr, v), kTaOne, kTaMagic));
+        }
+        // bytes 0, 1 and 2 of the four rows
+        const uint32_t a = __byte_perm(f[0], f[1], 0x5140), b = __byte_perm(f[2], f[3], 0x5140);
+        w[r0 / 4] = __byte_perm(a, b, 0x5410);
+        w[NR / 4 + r0 / 4] = __byte_perm(a, b, 0x7632);
+        w[NR / 2 + r0 / 4] = __byte_perm(__byte_perm(f[0], f[1], 0x0062), __byte_perm(f[2], f[3], 0x0062), 0x5410);
+      }
+#pragma unroll
+      for (int g = 0; g < N / 16; ++g)
+        *reinterpret_cast<uint4 *>(sm.p + g * 2048 + tid * 16) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+      fence_proxy_async();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ta_arrive(&sm.pready);
+    }
+    if (n > 0) {
+      ta_wait(sm, &sm.ofull, (unsigned)((n - 1) & 1));
+      __syncwarp();
+      tc_fence_after();
+      fold((n - 1) & 1);
+    }
+    tc_fence_before();
+    // sums over the keys: one row per lane
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float t = warp_sum(l[r]);
+      if (lane == r) sm.lsum[warp][r] = t;
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Sh::kTmem);  // before the cluster waits: a CTA that waits for TMEM never waits for this one
+  }
+  const bool failed = sm.abort != 0;
+  if (failed && tid == 0 && p.r.bad_flag) atomicMax(p.r.bad_flag, -QASR_ERR_TIMEOUT);
+
+  // Row r is finished by CTA r % C; partial states go there.
+  if (C > 1) cluster_wait_all();
+  if (warp < 4) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      if (r >= rows) break;
+      const uint32_t to = C > 1 ? cluster_map(smem_u32(&sm.recv[r / C * C + rank][tid]), r % C)
+                                : smem_u32(&sm.recv[r][tid]);
+      ta_store_remote(to, acc[r]);
+    }
+    if (warp == 0 && lane < rows) {
+      const float t = __fadd_rn(__fadd_rn(sm.lsum[0][lane], sm.lsum[1][lane]),
+                                __fadd_rn(sm.lsum[2][lane], sm.lsum[3][lane]));
+      const float mm = failed ? __uint_as_float(0x7fc00000u) : m_run;
+      uint32_t am = smem_u32(&sm.recv_m[lane / C * C + rank]), al = smem_u32(&sm.recv_l[lane / C * C + rank]);
+      if (C > 1) am = cluster_map(am, lane % C), al = cluster_map(al, lane % C);
+      ta_store_remote(am, mm);
+      ta_store_remote(al, failed ? mm : t);
+    }
+  }
+  __syncwarp();
+  if (C > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  if (warp < 4) {
+    for (int r = rank; r < rows; r += C) {
+      float top = -INFINITY;
+      const int e0 = r / C * C;
+      for (int c = 0; c < C; ++c) top = fmaxf(top, sm.recv_m[e0 + c]);
+      float sum = 0.0f, o = 0.0f;
+      for (int c = 0; c < C; ++c) {
+        const float mc = sm.recv_m[e0 + c];
+        const float f = mc == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(mc, top));
+        // a part that saw nothing counts as zero, unless its sum says otherwise (NaN seen)
+        sum = __fadd_rn(sum, mc == -INFINITY ? sm.recv_l[e0 + c] : __fmul_rn(sm.recv_l[e0 + c], f));
+        o = mc == -INFINITY ? o : fmaf(sm.recv[e0 + c][tid], f, o);
+      }
+      const int v = v0 + r, t = v / W, h = v % W, d = tid - h / G * HD;
+      if (d >= 0 && d < HD && hb * W + h < p.n_heads)
+        p.out[((size_t)(s.row0 + t) * p.n_heads + hb * W + h) * HD + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
+    }
+  }
+}
+
+template <int HD, int NR>
+static int tree_attention_launch(const TreeAttnParams &p, cudaStream_t st) {
+  constexpr int HPB = 128 / HD;
+  const size_t smem = sizeof(TaSmem<NR>) + 1024;
+  static bool attr_done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return QASR_ERR_INVALID;
+  if (!attr_done[dev]) {
+    int rc = cuda_status(cudaFuncSetAttribute(tree_attention_kernel<HD, NR>,
+                                              cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                         "qasr_tree_attention_int8: shared memory opt-in");
+    if (!rc)
+      rc = cuda_status(cudaFuncSetAttribute(tree_attention_kernel<HD, NR>,
+                                            cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                       "qasr_tree_attention_int8: cluster size opt-in");
+    if (rc) return rc;
+    attr_done[dev] = true;
+  }
+  const int W = HPB * (p.n_heads / p.c.n_kv_heads);
+  const long blocks = (long)ceil_div(p.c.n_kv_heads, HPB) * ceil_div((long)p.r.max_rows * W, NR);
+  if (blocks > 65535) {
+    set_error("qasr_tree_attention_int8: too many query rows per sequence (%d)", p.r.max_rows);
+    return QASR_ERR_UNSUPPORTED;
+  }
+  // CTAs per block of rows: enough to fill two per SM, no more than the cache has tiles
+  int C = 1;
+  const int tiles = ceil_div(p.c.max_seq, kTaKeys);
+  while (C < kTaMaxCluster && C < tiles && blocks * p.r.n_seqs * C < 148) C *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)C, (unsigned)blocks, (unsigned)p.r.n_seqs);
+  cfg.blockDim = dim3(kTaThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, tree_attention_kernel<HD, NR>, p), "qasr_tree_attention_int8");
+}
+
+template <int HD>
+static int tree_attention_rows(const TreeAttnParams &p, cudaStream_t st) {
+  const long rows = (long)p.r.max_rows * (128 / HD) * (p.n_heads / p.c.n_kv_heads);
+  if (rows <= 4) return tree_attention_launch<HD, 4>(p, st);
+  if (rows <= 8) return tree_attention_launch<HD, 8>(p, st);
+  if (rows <= 16) return tree_attention_launch<HD, 16>(p, st);
+  return tree_attention_launch<HD, 32>(p, st);
+}
+
+// Codes as a [cache rows, kv_dim] byte matrix.
+static int kv_codes_map(CUtensorMap *tm, const int8_t *codes, const qasr_kv_int8 &c) {
+  const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+  if (!encode) return QASR_ERR_CUDA;
+  const cuuint64_t kv_dim = (cuuint64_t)c.n_kv_heads * c.head_dim;
+  const cuuint64_t dims[2] = {kv_dim, (cuuint64_t)c.n_slots * c.n_layers * c.max_seq};
+  const cuuint64_t strides[1] = {kv_dim};
+  const cuuint32_t box[2] = {128, kTaKeys};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(codes), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("qasr_tree_attention_int8: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return QASR_ERR_CUDA;
+  }
+  return QASR_OK;
 }
 
 }  // namespace qasr
@@ -115,12 +655,17 @@ extern "C" int qasr_tree_attention_int8(float *out, const float *q, const qasr_k
     return QASR_ERR_UNSUPPORTED;
   }
   if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return QASR_OK;
-  const TreeAttnParams p{out, q, *cache, *rows, tree_mask, layer, n_heads, scale};
-  const dim3 grid((unsigned)ceil_div(rows->max_rows, 4), (unsigned)n_heads, (unsigned)rows->n_seqs);
+  TreeAttnParams p{};
+  if (int rc = kv_codes_map(&p.tm_k, cache->k, *cache)) return rc;
+  if (int rc = kv_codes_map(&p.tm_v, cache->v, *cache)) return rc;
+  p.out = out;
+  p.q = q;
+  p.c = *cache;
+  p.r = *rows;
+  p.tree_mask = tree_mask;
+  p.layer = layer;
+  p.n_heads = n_heads;
+  p.scale = scale;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (cache->head_dim == 128)
-    tree_attention_kernel<128><<<grid, 128, 0, st>>>(p);
-  else
-    tree_attention_kernel<64><<<grid, 128, 0, st>>>(p);
-  return launch_status("qasr_tree_attention_int8");
+  return cache->head_dim == 128 ? tree_attention_rows<128>(p, st) : tree_attention_rows<64>(p, st);
 }
