@@ -110,7 +110,7 @@ struct TaShape {
   static constexpr int kN = NR == 4 ? 16 : NR == 8 ? 32 : 3 * NR;
   static constexpr int kTmem = NR == 32 ? 256 : NR == 16 ? 128 : NR == 8 ? 64 : 32;  // S and O, a power of two
   static constexpr int kStages = NR <= 8 ? 3 : 2;  // K and V tiles in flight
-  static constexpr int kChunk = NR < 16 ? NR : 16;  // rows per TMEM load
+  static constexpr int kChunk = NR < 16 ? NR : NR == 16 ? 16 : 8;  // rows per TMEM load (fewer spills at 32 rows)
   static constexpr int kQBytes = kN * 128, kPBytes = kN * 128;
 };
 
@@ -138,10 +138,11 @@ struct TaSmem {
   float wvs[2][4][2];     // ... and largest value scales
   float qf[NR];           // 2^(E-22) * scale * log2(e)
   float lsum[4][NR];
-  uint64_t mask[NR];
+  uint32_t mask[2][NR];
   int tok[NR];            // the row's token, -1 for none
+  long long at[NR];       // element of q and out where value column 0 of the row's tile falls
   uint64_t full_k[3], full_v[3], empty[3], sfull, sfree, pready, ofull, qready, done;
-  uint32_t tmem;
+  uint32_t tmem, hi;
   int abort;
 };
 
@@ -222,17 +223,29 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
   const int C = gridDim.x, rank = blockIdx.x, m = blockIdx.z;
   const int G = p.n_heads / p.c.n_kv_heads, W = HPB * G;  // query rows of one token in a block
   const int hblocks = (p.c.n_kv_heads + HPB - 1) / HPB, hb = blockIdx.y % hblocks, rb = blockIdx.y / hblocks;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && m == 0 && warp == 5) kv_flag_bad(p.r, p.c, lane);
   const KvSeq s = kv_seq(p.r, p.c, m);
   const int v0 = rb * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
-  if (rows <= 0) return;                                 // the whole cluster
+  const bool first = blockIdx.x == 0 && blockIdx.y == 0 && m == 0;
+  if (rows <= 0) {  // the whole cluster
+    if (first && warp == 0) kv_flag_bad(p.r, p.c, lane);
+    return;
+  }
   const bool tree = p.tree_mask != nullptr;
   const int len = s.pos + (tree ? s.n : (v0 + rows - 1) / W + 1);  // keys any row may see
   const int tiles = (len + kTaKeys - 1) / kTaKeys;
   const int i0 = (int)((long)tiles * rank / C), n = (int)((long)tiles * (rank + 1) / C) - i0;
 
   if (C > 1) cluster_arrive_all();  // waited for before the first remote store: every CTA has started
-  if (tid == 0) {
+  // the first tiles are on their way before anything else is set up
+  const int row0 = (int)kv_row(p.c, s.slot, p.layer, 0);
+  auto fetch = [&](int i) {
+    const int st = i % ST, y = row0 + (i0 + i) * kTaKeys;
+    mbar_arrive_expect_tx(&sm.full_k[st], kTaTile);
+    tma_load_2d_u8(sm.ring[st][0], &p.tm_k, hb * 128, y, &sm.full_k[st]);
+    mbar_arrive_expect_tx(&sm.full_v[st], kTaTile);
+    tma_load_2d_u8(sm.ring[st][1], &p.tm_v, hb * 128, y, &sm.full_v[st]);
+  };
+  if (tid == 160) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&sm.full_k[i], 1);
       mbar_init(&sm.full_v[i], 1);
@@ -246,9 +259,11 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
     mbar_init(&sm.done, 1);
     sm.abort = 0;
     mbar_fence_init();
+    for (int i = 0; i < min(n, ST); ++i) fetch(i);
   }
   if (warp == 4) tmem_alloc(&sm.tmem, Sh::kTmem);
   tc_fence_before();
+  __syncwarp();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem, tmem_o = tmem + N;
@@ -259,17 +274,11 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
 
   if (warp == 5) {
     // ---------------------------------------------------------------- TMA
-    if (lane == 0 && n > 0) {
-      const int row = (int)kv_row(p.c, s.slot, p.layer, 0);
-      int i = 0;
+    if (lane == 0) {
+      int i = min(n, ST);
       for (; i < n; ++i) {
-        const int st = i % ST;
-        if (i >= ST && !ta_wait(sm, &sm.empty[st], (unsigned)((i / ST - 1) & 1))) break;
-        const int y = row + (i0 + i) * kTaKeys;
-        mbar_arrive_expect_tx(&sm.full_k[st], kTaTile);
-        tma_load_2d_u8(sm.ring[st][0], &p.tm_k, hb * 128, y, &sm.full_k[st]);
-        mbar_arrive_expect_tx(&sm.full_v[st], kTaTile);
-        tma_load_2d_u8(sm.ring[st][1], &p.tm_v, hb * 128, y, &sm.full_v[st]);
+        if (!ta_wait(sm, &sm.empty[i % ST], (unsigned)((i / ST - 1) & 1))) break;
+        fetch(i);
       }
       // copies that nobody waited for (after a timeout) land before the CTA leaves
       for (int k = max(0, i - ST); k < i; ++k) {
@@ -277,6 +286,8 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
         mbar_wait(&sm.full_v[k % ST], (unsigned)((k / ST) & 1));
       }
     }
+    __syncwarp();
+    if (first) kv_flag_bad(p.r, p.c, lane);
   } else if (warp == 4) {
     // ---------------------------------------------------------------- MMA
     if (lane == 0 && n > 0) {
@@ -313,24 +324,42 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
     }
   } else {
     // ------------------------------------------------------------ softmax
-    for (int r = warp; r < NR; r += 4) {
-      const int v = v0 + r, t = r < rows ? v / W : -1, h = v % W, b = 4 * lane - h / G * HD;  // b: value of the head
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (t >= 0 && b >= 0 && b < HD && hb * W + h < p.n_heads)
-        x = *reinterpret_cast<const float4 *>(p.q + ((size_t)(s.row0 + t) * p.n_heads + hb * W + h) * HD + b);
+    // lane r: row r's token, place in q and out, and half of the tile (pairs of heads)
+    const int v = v0 + lane, t = lane < rows ? v / W : -1, h = v % W;
+    const uint32_t hi = HPB == 2 ? __ballot_sync(0xffffffffu, lane < NR && h >= G) : 0;  // bit r: the second head
+    const bool live = t >= 0 && hb * W + h < p.n_heads;
+    const long long at =
+        live ? ((long long)(s.row0 + t) * p.n_heads + hb * W + h - (HPB == 2 && h >= G)) * HD : -1;
+    float4 x4[NR / 4];
+#pragma unroll
+    for (int k = 0; k < NR / 4; ++k) {  // warp w converts rows w, w + 4, ..: all their loads in flight
+      const int r = warp + 4 * k, b = 4 * lane, b0 = HPB == 2 && (hi >> r & 1) ? HD : 0;
+      const long long a = __shfl_sync(0xffffffffu, at, r);
+      x4[k] = a >= 0 && b >= b0 && b < b0 + HD ? *reinterpret_cast<const float4 *>(p.q + a + b)
+                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (warp == 0 && lane < NR) {
+      const uint64_t mask = t >= 0 && tree ? p.tree_mask[s.row0 + t] : 0;
+      sm.mask[0][lane] = (uint32_t)mask;
+      sm.mask[1][lane] = (uint32_t)(mask >> 32);
+      sm.tok[lane] = t;
+      sm.at[lane] = at;
+      if (lane == 0) sm.hi = hi;
+    }
+#pragma unroll
+    for (int k = 0; k < NR / 4; ++k) {
+      const float4 x = x4[k];
       constexpr uint32_t kAbs = 0x7fffffffu;
       const uint32_t top = __reduce_max_sync(
           0xffffffffu, max(max(__float_as_uint(x.x) & kAbs, __float_as_uint(x.y) & kAbs),
                            max(__float_as_uint(x.z) & kAbs, __float_as_uint(x.w) & kAbs)));
-      // 2^E above the largest magnitude; below 2^-100 the scores are as good as zero.  NaN or an infinity
+      // 2^e above the largest magnitude; below 2^-100 the scores are as good as zero.  NaN or an infinity
       // (all exponent bits) makes the row's factor, and so its scores, NaN.
       const int e = max((int)(top >> 23) - 126, -100);
-      ta_put_digits<NR>(sm.q, r, 4 * lane, x, __int_as_float((127 + 22 - e) << 23));
+      ta_put_digits<NR>(sm.q, warp + 4 * k, 4 * lane, x, __int_as_float((127 + 22 - e) << 23));
       if (lane == 0) {
         const float f = __fmul_rn(__int_as_float((127 + e - 22) << 23), __fmul_rn(p.scale, 1.44269504088896341f));
-        sm.qf[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : f;
-        sm.tok[r] = t;
-        sm.mask[r] = t >= 0 && tree ? p.tree_mask[s.row0 + t] : 0;
+        sm.qf[warp + 4 * k] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : f;
       }
     }
     for (int b = 3 * NR * 128 + 4 * tid; b < Sh::kQBytes; b += 512) *reinterpret_cast<uint32_t *>(sm.q + b) = 0;
@@ -350,13 +379,6 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
         nvs[u] = in ? __ldg(p.c.v_scales + at) : 0.0f;
       }
     };
-    // Second kv head of the pair for this row (HPB = 2).
-    auto second = [&](int r) { return HPB == 2 && (v0 + r) % W >= G; };
-    uint32_t hi = 0;  // bit r: row r is of the pair's second head
-    if constexpr (HPB == 2) {
-#pragma unroll
-      for (int r = 0; r < NR; ++r) hi |= second(r) ? 1u << r : 0u;
-    }
     // acc = acc * old + O * coef for the tile whose constants are in rowc[b]
     auto fold = [&](int b) {
 #pragma unroll
@@ -401,10 +423,16 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       if (lane == 0) ta_arrive(&sm.sfree);
       const int place = j - s.pos;  // >= 0: the row of one of the sequence's own tokens
       if ((i0 + i + 1) * kTaKeys > s.pos) {
+        if (tree) {
+          const bool in = place < s.n;
+          const int word = place >> 5 & 1, bit = place & 31;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const bool see = place < 0 || (place < s.n && (tree ? sm.mask[r] >> (place & 63) & 1 : place <= sm.tok[r]));
-          if (!see) x[r] = -INFINITY;
+          for (int r = 0; r < NR; ++r)
+            if (place >= 0 && !(in && sm.mask[word][r] >> bit & 1)) x[r] = -INFINITY;
+        } else {
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+            if (place > sm.tok[r] && place >= 0) x[r] = -INFINITY;
         }
       }
       // a value scale that is no finite number >= 0 counts as NaN, for the rows that see it
@@ -491,12 +519,8 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       fold((n - 1) & 1);
     }
     tc_fence_before();
-    // sums over the keys: one row per lane
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      const float t = warp_sum(l[r]);
-      if (lane == r) sm.lsum[warp][r] = t;
-    }
+    // sums over the keys
+    sm.lsum[warp][reduce_index<NR>(lane)] = warp_reduce_scatter<NR>(l);
   }
   __syncwarp();
   __syncthreads();
@@ -507,48 +531,64 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
   const bool failed = sm.abort != 0;
   if (failed && tid == 0 && p.r.bad_flag) atomicMax(p.r.bad_flag, -QASR_ERR_TIMEOUT);
 
-  // Row r is finished by CTA r % C; partial states go there.
-  if (C > 1) cluster_wait_all();
+  float part_l = 0.0f;  // lane = row
+  if (warp < 4 && lane < NR)
+    part_l = failed ? __uint_as_float(0x7fc00000u)
+                    : __fadd_rn(__fadd_rn(sm.lsum[0][lane], sm.lsum[1][lane]),
+                                __fadd_rn(sm.lsum[2][lane], sm.lsum[3][lane]));
+  if (C == 1) {
+    if (warp < 4) {
+      const float inv = part_l == 0.0f ? 0.0f : __fdiv_rn(1.0f, part_l);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float f = __shfl_sync(0xffffffffu, inv, r);
+        const long long at = sm.at[r];
+        const bool mine = HPB == 1 || (tid >= HD) == (sm.hi >> r & 1);
+        if (at >= 0 && mine) p.out[at + tid] = __fmul_rn(acc[r], f);
+      }
+    }
+    return;
+  }
+
+  // Row r is finished by CTA r % C (C is a power of two); partial states go there.
+  cluster_wait_all();
+  const int below = C - 1;
   if (warp < 4) {
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      if (r >= rows) break;
-      const uint32_t to = C > 1 ? cluster_map(smem_u32(&sm.recv[r / C * C + rank][tid]), r % C)
-                                : smem_u32(&sm.recv[r][tid]);
-      ta_store_remote(to, acc[r]);
-    }
+    for (int r = 0; r < NR; ++r)
+      if (r < rows) ta_store_remote(cluster_map(smem_u32(&sm.recv[(r & ~below) + rank][tid]), r & below), acc[r]);
     if (warp == 0 && lane < rows) {
-      const float t = __fadd_rn(__fadd_rn(sm.lsum[0][lane], sm.lsum[1][lane]),
-                                __fadd_rn(sm.lsum[2][lane], sm.lsum[3][lane]));
-      const float mm = failed ? __uint_as_float(0x7fc00000u) : m_run;
-      uint32_t am = smem_u32(&sm.recv_m[lane / C * C + rank]), al = smem_u32(&sm.recv_l[lane / C * C + rank]);
-      if (C > 1) am = cluster_map(am, lane % C), al = cluster_map(al, lane % C);
-      ta_store_remote(am, mm);
-      ta_store_remote(al, failed ? mm : t);
+      const int e = (lane & ~below) + rank;
+      ta_store_remote(cluster_map(smem_u32(&sm.recv_m[e]), lane & below), m_run);
+      ta_store_remote(cluster_map(smem_u32(&sm.recv_l[e]), lane & below), part_l);
     }
   }
   __syncwarp();
-  if (C > 1)
-    cluster_sync_all();
-  else
-    __syncthreads();
-  if (warp < 4) {
-    for (int r = rank; r < rows; r += C) {
-      float top = -INFINITY;
-      const int e0 = r / C * C;
-      for (int c = 0; c < C; ++c) top = fmaxf(top, sm.recv_m[e0 + c]);
-      float sum = 0.0f, o = 0.0f;
-      for (int c = 0; c < C; ++c) {
-        const float mc = sm.recv_m[e0 + c];
-        const float f = mc == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(mc, top));
-        // a part that saw nothing counts as zero, unless its sum says otherwise (NaN seen)
-        sum = __fadd_rn(sum, mc == -INFINITY ? sm.recv_l[e0 + c] : __fmul_rn(sm.recv_l[e0 + c], f));
-        o = mc == -INFINITY ? o : fmaf(sm.recv[e0 + c][tid], f, o);
-      }
-      const int v = v0 + r, t = v / W, h = v % W, d = tid - h / G * HD;
-      if (d >= 0 && d < HD && hb * W + h < p.n_heads)
-        p.out[((size_t)(s.row0 + t) * p.n_heads + hb * W + h) * HD + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
+  cluster_sync_all();
+  // one warp per row: lane c has part c's maximum and sum, then four columns of the output
+  for (int r = rank + warp * C; r < rows; r += C * (kTaThreads / 32)) {
+    const int e0 = r & ~below;
+    const float mc = lane < C ? sm.recv_m[e0 + lane] : -INFINITY, lc = lane < C ? sm.recv_l[e0 + lane] : 0.0f;
+    const float top = warp_max(mc);
+    // a part that saw nothing has sum 0 (NaN if it failed or saw a NaN) and counts as nothing
+    const float fc = mc == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(mc, top));
+    const float sum = warp_sum(mc == -INFINITY ? lc : __fmul_rn(lc, fc));
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < C; ++c) {
+      const float f = __shfl_sync(0xffffffffu, fc, c);
+      const float4 a = *reinterpret_cast<const float4 *>(&sm.recv[e0 + c][4 * lane]);
+      o.x = fmaf(a.x, f, o.x);
+      o.y = fmaf(a.y, f, o.y);
+      o.z = fmaf(a.z, f, o.z);
+      o.w = fmaf(a.w, f, o.w);
     }
+    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    const long long at = sm.at[r];
+    const bool mine = HPB == 1 || (4 * lane >= HD) == (sm.hi >> r & 1);
+    if (at >= 0 && mine)
+      *reinterpret_cast<float4 *>(p.out + at + 4 * lane) =
+          make_float4(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv), __fmul_rn(o.z, inv), __fmul_rn(o.w, inv));
   }
 }
 
