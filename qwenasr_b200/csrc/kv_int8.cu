@@ -88,6 +88,8 @@ kv_append_int8_kernel(const qasr_kv_int8 c, int layer, const qasr_kv_rows r, con
   const int lane = threadIdx.x & 31;
   const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int groups = (c.n_kv_heads + HPW - 1) / HPW;
+  pdl_launch_dependents();
+  pdl_wait();
   if (item == 0) kv_flag_bad(r, c, lane);
   if (item >= (long)r.n_rows * groups) return;
   const int row = (int)(item / groups), head = (int)(item % groups) * HPW + lane / LPH;
@@ -136,6 +138,8 @@ kv_read_int8_kernel(float *__restrict__ k_out, float *__restrict__ v_out, const 
   const int lane = threadIdx.x & 31;
   const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int groups = (c.n_kv_heads + HPW - 1) / HPW;
+  pdl_launch_dependents();
+  pdl_wait();
   if (item == 0) kv_flag_bad(r, c, lane);
   if (item >= (long)r.n_rows * groups) return;
   const int row = (int)(item / groups), head = (int)(item % groups) * HPW + lane / LPH;
@@ -170,11 +174,12 @@ extern "C" int qasr_kv_append_int8(const qasr_kv_int8 *cache, int layer, const q
   if (rows->n_seqs == 0 || rows->n_rows == 0) return QASR_OK;
   const int hpw = 128 / cache->head_dim;
   const unsigned grid = (unsigned)ceil_div((long)rows->n_rows * ceil_div(cache->n_kv_heads, hpw), 8);
+  cudaError_t e;
   if (cache->head_dim == 128)
-    kv_append_int8_kernel<128><<<grid, 256, 0, S(stream)>>>(*cache, layer, *rows, k_new, v_new, src_rows, n_src);
+    e = launch_pdl(kv_append_int8_kernel<128>, grid, 256, 0, S(stream), *cache, layer, *rows, k_new, v_new, src_rows, n_src);
   else
-    kv_append_int8_kernel<64><<<grid, 256, 0, S(stream)>>>(*cache, layer, *rows, k_new, v_new, src_rows, n_src);
-  return launch_status("qasr_kv_append_int8");
+    e = launch_pdl(kv_append_int8_kernel<64>, grid, 256, 0, S(stream), *cache, layer, *rows, k_new, v_new, src_rows, n_src);
+  return cuda_status(e, "qasr_kv_append_int8");
 }
 
 extern "C" int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 *cache, int layer,
@@ -187,9 +192,10 @@ extern "C" int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 
   if (rows->n_seqs == 0 || rows->n_rows == 0) return QASR_OK;
   const int hpw = 128 / cache->head_dim;
   const unsigned grid = (unsigned)ceil_div((long)rows->n_rows * ceil_div(cache->n_kv_heads, hpw), 8);
+  cudaError_t e;
   if (cache->head_dim == 128)
-    kv_read_int8_kernel<128><<<grid, 256, 0, S(stream)>>>(k_out, v_out, *cache, layer, *rows);
+    e = launch_pdl(kv_read_int8_kernel<128>, grid, 256, 0, S(stream), k_out, v_out, *cache, layer, *rows);
   else
-    kv_read_int8_kernel<64><<<grid, 256, 0, S(stream)>>>(k_out, v_out, *cache, layer, *rows);
-  return launch_status("qasr_kv_read_int8");
+    e = launch_pdl(kv_read_int8_kernel<64>, grid, 256, 0, S(stream), k_out, v_out, *cache, layer, *rows);
+  return cuda_status(e, "qasr_kv_read_int8");
 }

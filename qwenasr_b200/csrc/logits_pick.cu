@@ -41,6 +41,8 @@ QASR_DEV void pick_list(const int32_t *starts, int n, int m, int32_t *bad, int &
 __global__ void __launch_bounds__(kPickThreads) logits_pick_kernel(const PickParams p) {
   __shared__ __align__(16) uint32_t s_count[kPickTile], s_bias[kPickTile];
   __shared__ unsigned long long s_warp[kPickThreads / 32], s_rank[kPickCluster];
+  pdl_launch_dependents();
+  pdl_wait();
   cluster_arrive_all();  // every CTA of the cluster has started before one writes to another
   const int rank = (int)cluster_ctarank(), m = blockIdx.y, V = p.vocab;
   const qasr_pick_rules &r = p.r;
@@ -171,11 +173,13 @@ extern "C" int qasr_logits_pick(int32_t *ids, float *logits_out, const float *lo
   cfg.gridDim = dim3(kPickCluster, (unsigned)M);
   cfg.blockDim = dim3(kPickThreads);
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kPickCluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kPickCluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cuda_status(cudaLaunchKernelEx(&cfg, logits_pick_kernel, p), "qasr_logits_pick");
 }

@@ -223,28 +223,7 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
   const int C = gridDim.x, rank = blockIdx.x, m = blockIdx.z;
   const int G = p.n_heads / p.c.n_kv_heads, W = HPB * G;  // query rows of one token in a block
   const int hblocks = (p.c.n_kv_heads + HPB - 1) / HPB, hb = blockIdx.y % hblocks, rb = blockIdx.y / hblocks;
-  const KvSeq s = kv_seq(p.r, p.c, m);
-  const int v0 = rb * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
-  const bool first = blockIdx.x == 0 && blockIdx.y == 0 && m == 0;
-  if (rows <= 0) {  // the whole cluster
-    if (first && warp == 0) kv_flag_bad(p.r, p.c, lane);
-    return;
-  }
-  const bool tree = p.tree_mask != nullptr;
-  const int len = s.pos + (tree ? s.n : (v0 + rows - 1) / W + 1);  // keys any row may see
-  const int tiles = (len + kTaKeys - 1) / kTaKeys;
-  const int i0 = (int)((long)tiles * rank / C), n = (int)((long)tiles * (rank + 1) / C) - i0;
-
-  if (C > 1) cluster_arrive_all();  // waited for before the first remote store: every CTA has started
-  // the first tiles are on their way before anything else is set up
-  const int row0 = (int)kv_row(p.c, s.slot, p.layer, 0);
-  auto fetch = [&](int i) {
-    const int st = i % ST, y = row0 + (i0 + i) * kTaKeys;
-    mbar_arrive_expect_tx(&sm.full_k[st], kTaTile);
-    tma_load_2d_u8(sm.ring[st][0], &p.tm_k, hb * 128, y, &sm.full_k[st]);
-    mbar_arrive_expect_tx(&sm.full_v[st], kTaTile);
-    tma_load_2d_u8(sm.ring[st][1], &p.tm_v, hb * 128, y, &sm.full_v[st]);
-  };
+  // what does not depend on the kernel before: barriers, tensor memory
   if (tid == 160) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&sm.full_k[i], 1);
@@ -259,7 +238,6 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
     mbar_init(&sm.done, 1);
     sm.abort = 0;
     mbar_fence_init();
-    for (int i = 0; i < min(n, ST); ++i) fetch(i);
   }
   if (warp == 4) tmem_alloc(&sm.tmem, Sh::kTmem);
   tc_fence_before();
@@ -267,6 +245,22 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem, tmem_o = tmem + N;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const KvSeq s = kv_seq(p.r, p.c, m);
+  const int v0 = rb * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
+  const bool first = blockIdx.x == 0 && blockIdx.y == 0 && m == 0;
+  if (rows <= 0) {  // the whole cluster
+    if (first && warp == 0) kv_flag_bad(p.r, p.c, lane);
+    if (warp == 4) tmem_dealloc(tmem, Sh::kTmem);
+    return;
+  }
+  const bool tree = p.tree_mask != nullptr;
+  const int len = s.pos + (tree ? s.n : (v0 + rows - 1) / W + 1);  // keys any row may see
+  const int tiles = (len + kTaKeys - 1) / kTaKeys;
+  const int i0 = (int)((long)tiles * rank / C), n = (int)((long)tiles * (rank + 1) / C) - i0;
+  if (C > 1) cluster_arrive_all();  // waited for before the first remote store: every CTA has started
 
   float acc[NR], l[NR], m_run = -INFINITY;  // thread = value column (acc), key (l); lane = row (m_run)
 #pragma unroll
@@ -275,10 +269,15 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
   if (warp == 5) {
     // ---------------------------------------------------------------- TMA
     if (lane == 0) {
-      int i = min(n, ST);
+      const int row = (int)kv_row(p.c, s.slot, p.layer, 0);
+      int i = 0;
       for (; i < n; ++i) {
-        if (!ta_wait(sm, &sm.empty[i % ST], (unsigned)((i / ST - 1) & 1))) break;
-        fetch(i);
+        const int st = i % ST, y = row + (i0 + i) * kTaKeys;
+        if (i >= ST && !ta_wait(sm, &sm.empty[st], (unsigned)((i / ST - 1) & 1))) break;
+        mbar_arrive_expect_tx(&sm.full_k[st], kTaTile);
+        tma_load_2d_u8(sm.ring[st][0], &p.tm_k, hb * 128, y, &sm.full_k[st]);
+        mbar_arrive_expect_tx(&sm.full_v[st], kTaTile);
+        tma_load_2d_u8(sm.ring[st][1], &p.tm_v, hb * 128, y, &sm.full_v[st]);
       }
       // copies that nobody waited for (after a timeout) land before the CTA leaves
       for (int k = max(0, i - ST); k < i; ++k) {
@@ -626,12 +625,14 @@ static int tree_attention_launch(const TreeAttnParams &p, cudaStream_t st) {
   cfg.blockDim = dim3(kTaThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)C;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)C;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = C > 1 ? 1 : 0;
+  cfg.numAttrs = C > 1 ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, tree_attention_kernel<HD, NR>, p), "qasr_tree_attention_int8");
 }
 

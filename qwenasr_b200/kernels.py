@@ -266,28 +266,35 @@ def final_norm_lmhead_argmax(ids_out, logits_out, x, norm_w, w, scales, M, hidde
 
 
 # ---------------------------------------------------------------- serving --
-def _need(t, dtype, device, name, numel):
-    """_ptr for an operand that must also lie on `device`."""
+def _need(t, dtype, dev, name, numel):
+    """Address of an operand: contiguous, on device index `dev`, of `dtype`, with `numel` elements at least.
+    These calls are short and a step makes several per layer, so the checks run once, without _ptr's objects."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise ValueError(f"{name} must be a tensor on {device}")
-    return _ptr(t, dtype, name, numel)
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+        raise ValueError(f"{name} must be a CUDA tensor on cuda:{dev}")
+    if t.dtype is not dtype or not t.is_contiguous() or t.numel() < numel:
+        _ptr(t, dtype, name, numel)  # raises with the reason
+    return t.data_ptr()
 
 
-def _on(device, name, *args):
-    """Call an entry on `device`, on that device's current stream (the last argument)."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, _stream())
+# The current stream's handle by device index, without a Stream object (several times the cost of the rest of a call).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _on(dev, name, *args):
+    """Call an entry on device index `dev`, on that device's current stream (the last argument)."""
+    if torch.cuda.current_device() == dev:
+        _lib.call(name, *args, _raw_stream(dev))
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, _stream())
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _raw_stream(dev))
 
 
 def _kv_args(cache, rows):
     if rows.device != cache.device:
         raise ValueError(f"rows are on {rows.device}, the cache on {cache.device}")
-    return cache.device, rows.n_rows
+    return cache.device.index, rows.n_rows
 
 
 def kv_append_int8(cache, layer, rows, k_new, v_new, src_rows=None):
@@ -329,10 +336,10 @@ def logits_pick(ids_out, logits_out, logits, M, vocab, history=None, history_sta
     starts [M + 1]; allow_mask is int32 [M, ceil(vocab / 32)], bit set = allowed."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
-    dev = logits.device
+    dev = logits.get_device()
 
     def opt(t, dtype, name, numel):
-        return None if t is None else _need(t, dtype, dev, name, numel).value
+        return _need(t, dtype, dev, name, numel)
 
     n_bias = 0 if bias_ids is None else bias_ids.numel()
     r = _lib.PickRules(opt(history, i32, "history", 0), opt(history_starts, i32, "history_starts", M + 1),
