@@ -97,7 +97,6 @@ QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][1
 
 constexpr int kTaKeys = 128;             // keys of a tile: TMEM lanes of S^T
 constexpr int kTaTile = kTaKeys * 128;   // bytes of a K (or V) tile
-constexpr int kTaThreads = 192;          // 4 softmax warps, the MMA warp, the TMA warp
 constexpr int kTaMaxCluster = 16;
 constexpr float kTaOne = 8388607.0f;     // a weight of 1
 constexpr float kTaMagic = 8388608.0f;   // 2^23: its low three bytes are zero
@@ -110,7 +109,10 @@ struct TaShape {
   static constexpr int kN = NR == 4 ? 16 : NR == 8 ? 32 : 3 * NR;
   static constexpr int kTmem = NR == 32 ? 256 : NR == 16 ? 128 : NR == 8 ? 64 : 32;  // S and O, a power of two
   static constexpr int kStages = NR <= 8 ? 3 : 2;  // K and V tiles in flight
-  static constexpr int kChunk = NR < 16 ? NR : NR == 16 ? 16 : 8;  // rows per TMEM load (fewer spills at 32 rows)
+  static constexpr int kGroups = NR == 32 ? 2 : 1;  // softmax warpgroups: each owns R rows of every tile
+  static constexpr int kR = NR / kGroups;
+  static constexpr int kChunk = kGroups > 1 ? 8 : kR;  // rows per TMEM load: eight spill less at 96 registers
+  static constexpr int kWarps = 4 * kGroups, kThreads = 32 * kWarps + 64;  // and the MMA and the TMA warp
   static constexpr int kQBytes = kN * 128, kPBytes = kN * 128;
 };
 
@@ -122,22 +124,25 @@ struct TreeAttnParams {
   qasr_kv_rows r;
   const uint64_t *tree_mask;
   int layer, n_heads;
+  int group, width;  // query heads per kv head; query rows of one token in a block (group x heads per tile)
+  int cshift;        // log2 of the cluster size
   float scale;
 };
 
 template <int NR>
 struct TaSmem {
-  alignas(1024) unsigned char ring[TaShape<NR>::kStages][2][kTaTile];  // K, V
-  alignas(1024) unsigned char q[TaShape<NR>::kQBytes];  // digits, K-major, 128-byte swizzle
-  alignas(1024) unsigned char p[TaShape<NR>::kPBytes];  // digits, N-major, no swizzle
+  using Sh = TaShape<NR>;
+  alignas(1024) unsigned char ring[Sh::kStages][2][kTaTile];  // K, V
+  alignas(1024) unsigned char q[Sh::kQBytes];  // digits, K-major, 128-byte swizzle
+  alignas(1024) unsigned char p[Sh::kPBytes];  // digits, N-major, no swizzle
   // partial states pushed by the cluster: entry r / C * C + c is CTA c's of row r, one of the rows r % C = rank
   static constexpr int kRecv = NR < kTaMaxCluster ? kTaMaxCluster : NR;
   float recv[kRecv][128], recv_m[kRecv], recv_l[kRecv];
-  float4 rowc[2][4][NR];  // per tile (two in flight) and warp: tile maximum, factors of the new and old sums, of O
-  float wmax[2][4][NR];   // per tile and warp: row maxima
-  float wvs[2][4][2];     // ... and largest value scales
+  float4 rowc[2][Sh::kWarps][Sh::kR];  // per tile (two in flight) and warp: tile maximum, factors of the new and old sums, of O
+  float wmax[2][Sh::kWarps][Sh::kR];  // per tile and warp: row maxima
+  float wvs[2][Sh::kWarps][2];        // ... and largest value scales
   float qf[NR];           // 2^(E-22) * scale * log2(e)
-  float lsum[4][NR];
+  float lsum[4][NR], mrun[NR];
   uint32_t mask[2][NR];
   int tok[NR];            // the row's token, -1 for none
   long long at[NR];       // element of q and out where value column 0 of the row's tile falls
@@ -211,35 +216,36 @@ QASR_DEV void ta_put_digits(unsigned char *q, int r, int b, float4 v, float qm) 
   }
 }
 
-// HD: head_dim; HPB = 128 / HD kv heads share a tile.  Grid: (C, head blocks x
+// HD: head_dim; HPB = 128 / HD kv heads share a tile.  Grid: (C x head blocks,
 // row blocks, sequences), clusters of C along x.
 template <int HD, int NR>
-__global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
+__global__ void __launch_bounds__(TaShape<NR>::kThreads, 2)
+tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
   using Sh = TaShape<NR>;
-  constexpr int HPB = 128 / HD, N = Sh::kN, ST = Sh::kStages, CH = Sh::kChunk;
+  constexpr int HPB = 128 / HD, N = Sh::kN, ST = Sh::kStages, R = Sh::kR, CH = Sh::kChunk;
+  constexpr int kMmaWarp = Sh::kWarps, kTmaWarp = Sh::kWarps + 1;
   extern __shared__ unsigned char smem_raw[];
   TaSmem<NR> &sm = *reinterpret_cast<TaSmem<NR> *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int C = gridDim.x, rank = blockIdx.x, m = blockIdx.z;
-  const int G = p.n_heads / p.c.n_kv_heads, W = HPB * G;  // query rows of one token in a block
-  const int hblocks = (p.c.n_kv_heads + HPB - 1) / HPB, hb = blockIdx.y % hblocks, rb = blockIdx.y / hblocks;
+  const int C = 1 << p.cshift, rank = blockIdx.x & (C - 1), hb = blockIdx.x >> p.cshift, m = blockIdx.z;
+  const int G = p.group, W = p.width;
   // what does not depend on the kernel before: barriers, tensor memory
-  if (tid == 160) {
+  if (warp == kTmaWarp && lane == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&sm.full_k[i], 1);
       mbar_init(&sm.full_v[i], 1);
       mbar_init(&sm.empty[i], 1);
     }
     mbar_init(&sm.sfull, 1);
-    mbar_init(&sm.sfree, 4);
-    mbar_init(&sm.pready, 4);
+    mbar_init(&sm.sfree, Sh::kWarps);
+    mbar_init(&sm.pready, Sh::kWarps);
     mbar_init(&sm.ofull, 1);
-    mbar_init(&sm.qready, 4);
+    mbar_init(&sm.qready, 1);
     mbar_init(&sm.done, 1);
     sm.abort = 0;
     mbar_fence_init();
   }
-  if (warp == 4) tmem_alloc(&sm.tmem, Sh::kTmem);
+  if (warp == kMmaWarp) tmem_alloc(&sm.tmem, Sh::kTmem);
   tc_fence_before();
   __syncwarp();
   __syncthreads();
@@ -249,24 +255,25 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
   pdl_wait();
 
   const KvSeq s = kv_seq(p.r, p.c, m);
-  const int v0 = rb * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
+  const int v0 = blockIdx.y * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
   const bool first = blockIdx.x == 0 && blockIdx.y == 0 && m == 0;
   if (rows <= 0) {  // the whole cluster
     if (first && warp == 0) kv_flag_bad(p.r, p.c, lane);
-    if (warp == 4) tmem_dealloc(tmem, Sh::kTmem);
+    if (warp == kMmaWarp) tmem_dealloc(tmem, Sh::kTmem);
     return;
   }
   const bool tree = p.tree_mask != nullptr;
   const int len = s.pos + (tree ? s.n : (v0 + rows - 1) / W + 1);  // keys any row may see
-  const int tiles = (len + kTaKeys - 1) / kTaKeys;
-  const int i0 = (int)((long)tiles * rank / C), n = (int)((long)tiles * (rank + 1) / C) - i0;
+  const unsigned tiles = (unsigned)(len + kTaKeys - 1) / kTaKeys;  // < 2^25: times a rank still fits
+  const int i0 = (int)(tiles * rank >> p.cshift), n = (int)(tiles * (rank + 1) >> p.cshift) - i0;
   if (C > 1) cluster_arrive_all();  // waited for before the first remote store: every CTA has started
 
-  float acc[NR], l[NR], m_run = -INFINITY;  // thread = value column (acc), key (l); lane = row (m_run)
+  float acc[R], l[R], m_run = -INFINITY;  // thread = value column (acc), key (l); lane = row (m_run)
 #pragma unroll
-  for (int r = 0; r < NR; ++r) acc[r] = l[r] = 0.0f;
+  for (int r = 0; r < R; ++r) acc[r] = l[r] = 0.0f;
+  const int col = tid & 127, wg = warp >> 2;  // softmax warps: key / value column, first row wg * R
 
-  if (warp == 5) {
+  if (warp == kTmaWarp) {
     // ---------------------------------------------------------------- TMA
     if (lane == 0) {
       const int row = (int)kv_row(p.c, s.slot, p.layer, 0);
@@ -287,7 +294,7 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
     }
     __syncwarp();
     if (first) kv_flag_bad(p.r, p.c, lane);
-  } else if (warp == 4) {
+  } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- MMA
     if (lane == 0 && n > 0) {
       const uint32_t qa = smem_u32(sm.q), pa = smem_u32(sm.p);
@@ -324,18 +331,18 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
   } else {
     // ------------------------------------------------------------ softmax
     // lane r: row r's token, place in q and out, and half of the tile (pairs of heads)
-    const int v = v0 + lane, t = lane < rows ? v / W : -1, h = v % W;
-    const uint32_t hi = HPB == 2 ? __ballot_sync(0xffffffffu, lane < NR && h >= G) : 0;  // bit r: the second head
+    const int v = v0 + lane, t = lane < rows ? v / W : -1, h = v - t * W;
+    const uint32_t hi = HPB == 2 ? __ballot_sync(0xffffffffu, lane < rows && h >= G) : 0;  // bit r: the second head
     const bool live = t >= 0 && hb * W + h < p.n_heads;
-    const long long at =
-        live ? ((long long)(s.row0 + t) * p.n_heads + hb * W + h - (HPB == 2 && h >= G)) * HD : -1;
-    float4 x4[NR / 4];
+    const long long at = live ? ((long long)(s.row0 + t) * p.n_heads + hb * W + h - (HPB == 2 && h >= G)) * HD : -1;
+    constexpr int kQ = NR / Sh::kWarps;
+    float4 x4[kQ];
 #pragma unroll
-    for (int k = 0; k < NR / 4; ++k) {  // warp w converts rows w, w + 4, ..: all their loads in flight
-      const int r = warp + 4 * k, b = 4 * lane, b0 = HPB == 2 && (hi >> r & 1) ? HD : 0;
+    for (int k = 0; k < kQ; ++k) {  // warp w converts rows w, w + warps, ..: all their loads in flight
+      const int r = warp + Sh::kWarps * k, b = 4 * lane, b0 = HPB == 2 && (hi >> r & 1) ? HD : 0;
       const long long a = __shfl_sync(0xffffffffu, at, r);
       x4[k] = a >= 0 && b >= b0 && b < b0 + HD ? *reinterpret_cast<const float4 *>(p.q + a + b)
-                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+                                               : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (warp == 0 && lane < NR) {
       const uint64_t mask = t >= 0 && tree ? p.tree_mask[s.row0 + t] : 0;
@@ -346,7 +353,7 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       if (lane == 0) sm.hi = hi;
     }
 #pragma unroll
-    for (int k = 0; k < NR / 4; ++k) {
+    for (int k = 0; k < kQ; ++k) {
       const float4 x = x4[k];
       constexpr uint32_t kAbs = 0x7fffffffu;
       const uint32_t top = __reduce_max_sync(
@@ -354,22 +361,25 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
                            max(__float_as_uint(x.z) & kAbs, __float_as_uint(x.w) & kAbs)));
       // 2^e above the largest magnitude; below 2^-100 the scores are as good as zero.  NaN or an infinity
       // (all exponent bits) makes the row's factor, and so its scores, NaN.
-      const int e = max((int)(top >> 23) - 126, -100);
-      ta_put_digits<NR>(sm.q, warp + 4 * k, 4 * lane, x, __int_as_float((127 + 22 - e) << 23));
+      const int r = warp + Sh::kWarps * k, e = max((int)(top >> 23) - 126, -100);
+      ta_put_digits<NR>(sm.q, r, 4 * lane, x, __int_as_float((127 + 22 - e) << 23));
       if (lane == 0) {
         const float f = __fmul_rn(__int_as_float((127 + e - 22) << 23), __fmul_rn(p.scale, 1.44269504088896341f));
-        sm.qf[warp + 4 * k] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : f;
+        sm.qf[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : f;
       }
     }
     for (int b = 3 * NR * 128 + 4 * tid; b < Sh::kQBytes; b += 512) *reinterpret_cast<uint32_t *>(sm.q + b) = 0;
     fence_proxy_async();
-    named_bar(1, 128);
-    if (lane == 0) ta_arrive(&sm.qready);
-    const uint32_t my_s = tmem + ((uint32_t)warp << 21), my_o = tmem_o + ((uint32_t)warp << 21);
+    named_bar(1, 32 * Sh::kWarps);
+    if (tid == 0) ta_arrive(&sm.qready);
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21, my_s = tmem + lanes + wg * R, my_o = tmem_o + lanes + wg * R;
+    const uint32_t my_hi = hi >> (wg * R);  // bit r: the group's row r is of the pair's second head
+    const int *tok = sm.tok + wg * R;
+    const float *qf = sm.qf + wg * R;
     const size_t srow = kv_row(p.c, s.slot, p.layer, 0);
     float nks[HPB], nvs[HPB];  // scales of this thread's key of the next tile
     auto load_scales = [&](int i) {
-      const int j = (i0 + i) * kTaKeys + tid;
+      const int j = (i0 + i) * kTaKeys + col;
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
         const bool in = i < n && j < len && hb * HPB + u < p.c.n_kv_heads;
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
     // acc = acc * old + O * coef for the tile whose constants are in rowc[b]
     auto fold = [&](int b) {
 #pragma unroll
-      for (int c0 = 0; c0 < NR; c0 += CH) {
+      for (int c0 = 0; c0 < R; c0 += CH) {
         uint32_t d[3][CH];
         tmem_ld_planes(my_o + c0, NR, d);
 #pragma unroll
@@ -392,11 +402,11 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
         }
       }
     };
-    // After a timeout (sm.abort) every wait returns at once and the loop runs on: the four warps must meet at
+    // After a timeout (sm.abort) every wait returns at once and the loop runs on: a group's warps must meet at
     // the same number of barriers.  The results are thrown away.
     load_scales(0);
     for (int i = 0; i < n; ++i) {
-      const int buf = i & 1, j = (i0 + i) * kTaKeys + tid;
+      const int buf = i & 1, j = (i0 + i) * kTaKeys + col;
       float ks[HPB], vs[HPB];
 #pragma unroll
       for (int u = 0; u < HPB; ++u) ks[u] = nks[u], vs[u] = nvs[u];
@@ -404,17 +414,17 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       ta_wait(sm, &sm.sfull, (unsigned)(i & 1));
       __syncwarp();
       tc_fence_after();
-      float x[NR];  // scores in units of log 2
+      float x[R];  // scores in units of log 2
 #pragma unroll
-      for (int c0 = 0; c0 < NR; c0 += CH) {
+      for (int c0 = 0; c0 < R; c0 += CH) {
         uint32_t d[3][CH];
         tmem_ld_planes(my_s + c0, NR, d);
 #pragma unroll
         for (int e = 0; e < CH; ++e) {
           const int r = c0 + e;
-          const float k = HPB == 2 && (hi >> r & 1) ? ks[HPB - 1] : ks[0];
+          const float k = HPB == 2 && (my_hi >> r & 1) ? ks[HPB - 1] : ks[0];
           const float sum = fmaf((float)(int)d[0][e], 65536.0f, (float)((int)d[1][e] * 256 + (int)d[2][e]));
-          x[r] = __fmul_rn(sum, __fmul_rn(sm.qf[r], k));
+          x[r] = __fmul_rn(sum, __fmul_rn(qf[r], k));
         }
       }
       tc_fence_before();
@@ -423,15 +433,16 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       const int place = j - s.pos;  // >= 0: the row of one of the sequence's own tokens
       if ((i0 + i + 1) * kTaKeys > s.pos) {
         if (tree) {
+          const uint32_t *mask = sm.mask[place >> 5 & 1] + wg * R;
           const bool in = place < s.n;
-          const int word = place >> 5 & 1, bit = place & 31;
+          const int bit = place & 31;
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
-            if (place >= 0 && !(in && sm.mask[word][r] >> bit & 1)) x[r] = -INFINITY;
+          for (int r = 0; r < R; ++r)
+            if (place >= 0 && !(in && mask[r] >> bit & 1)) x[r] = -INFINITY;
         } else {
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
-            if (place > sm.tok[r] && place >= 0) x[r] = -INFINITY;
+          for (int r = 0; r < R; ++r)
+            if (place > tok[r] && place >= 0) x[r] = -INFINITY;
         }
       }
       // a value scale that is no finite number >= 0 counts as NaN, for the rows that see it
@@ -445,25 +456,27 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       }
       float mine = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
+      for (int r = 0; r < R; ++r) {
         const float t = ta_warp_max(x[r]);
         if (lane == r) mine = t;
       }
-      if (lane < NR) sm.wmax[buf][warp][lane] = mine;
-      named_bar(1, 128);
+      if (lane < R) sm.wmax[buf][warp][lane] = mine;
+      named_bar(2 + wg, 128);
+      const int w0 = 4 * wg;  // the group's warps
       float vmax[HPB];
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
-        vmax[u] = fmaxf(fmaxf(sm.wvs[buf][0][u], sm.wvs[buf][1][u]), fmaxf(sm.wvs[buf][2][u], sm.wvs[buf][3][u]));
+        vmax[u] = fmaxf(fmaxf(sm.wvs[buf][w0][u], sm.wvs[buf][w0 + 1][u]),
+                        fmaxf(sm.wvs[buf][w0 + 2][u], sm.wvs[buf][w0 + 3][u]));
         vs[u] = vmax[u] > 0.0f ? __fdiv_rn(vs[u], vmax[u]) : 0.0f;
       }
-      if (lane < NR) {
-        const float t = fmaxf(fmaxf(sm.wmax[buf][0][lane], sm.wmax[buf][1][lane]),
-                              fmaxf(sm.wmax[buf][2][lane], sm.wmax[buf][3][lane]));
+      if (lane < R) {
+        const float t = fmaxf(fmaxf(sm.wmax[buf][w0][lane], sm.wmax[buf][w0 + 1][lane]),
+                              fmaxf(sm.wmax[buf][w0 + 2][lane], sm.wmax[buf][w0 + 3][lane]));
         const float top = fmaxf(m_run, t), base = top == -INFINITY ? 0.0f : top;
         const float f = t == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(t, base));
         const float old = m_run == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(m_run, base));
-        const float vm = HPB == 2 && (hi >> lane & 1) ? vmax[HPB - 1] : vmax[0];
+        const float vm = HPB == 2 && (my_hi >> lane & 1) ? vmax[HPB - 1] : vmax[0];
         sm.rowc[buf][warp][lane] =
             make_float4(t == -INFINITY ? 0.0f : t, f, old, __fmul_rn(f, __fmul_rn(vm, 1.0f / kTaOne)));
         m_run = top;
@@ -473,8 +486,9 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       if constexpr (HPB == 2) any_odd |= odd[HPB - 1];
       if (__any_sync(0xffffffffu, any_odd)) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
-          if (x[r] != -INFINITY && (HPB == 2 && (hi >> r & 1) ? odd[HPB - 1] : odd[0])) l[r] = __uint_as_float(0x7fc00000u);
+        for (int r = 0; r < R; ++r)
+          if (x[r] != -INFINITY && (HPB == 2 && (my_hi >> r & 1) ? odd[HPB - 1] : odd[0]))
+            l[r] = __uint_as_float(0x7fc00000u);
       }
       if (i > 0) {  // the previous tile's O; its digits in sm.p are free after it
         ta_wait(sm, &sm.ofull, (unsigned)((i - 1) & 1));
@@ -482,11 +496,12 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
         tc_fence_after();
         fold(buf ^ 1);
       }
-      uint32_t w[3 * NR / 4 + (NR == 4 ? 1 : NR == 8 ? 2 : 0)];
-      w[3 * NR / 4 - 1 + (NR == 4 ? 1 : NR == 8 ? 2 : 0)] = 0;  // unused columns
-      if constexpr (NR == 8) w[6] = 0;
+      constexpr int kWords = R == 16 ? 12 : N / 4;  // of this thread's key: three planes of R bytes, then unused columns
+      uint32_t w[kWords];
 #pragma unroll
-      for (int r0 = 0; r0 < NR; r0 += 4) {
+      for (int r = 3 * R / 4; r < kWords; ++r) w[r] = 0;
+#pragma unroll
+      for (int r0 = 0; r0 < R; r0 += 4) {
         uint32_t f[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -494,18 +509,19 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
           const float4 c = sm.rowc[buf][warp][r];
           const float pr = ta_ex2(__fsub_rn(x[r], c.x));
           l[r] = fmaf(l[r], c.z, __fmul_rn(pr, c.y));
-          const float v = HPB == 2 && (hi >> r & 1) ? vs[HPB - 1] : vs[0];
+          const float v = HPB == 2 && (my_hi >> r & 1) ? vs[HPB - 1] : vs[0];
           f[e] = __float_as_uint(fmaf(__fmul_rn(pr, v), kTaOne, kTaMagic));
         }
         // bytes 0, 1 and 2 of the four rows
         const uint32_t a = __byte_perm(f[0], f[1], 0x5140), b = __byte_perm(f[2], f[3], 0x5140);
         w[r0 / 4] = __byte_perm(a, b, 0x5410);
-        w[NR / 4 + r0 / 4] = __byte_perm(a, b, 0x7632);
-        w[NR / 2 + r0 / 4] = __byte_perm(__byte_perm(f[0], f[1], 0x0062), __byte_perm(f[2], f[3], 0x0062), 0x5410);
+        w[R / 4 + r0 / 4] = __byte_perm(a, b, 0x7632);
+        w[R / 2 + r0 / 4] = __byte_perm(__byte_perm(f[0], f[1], 0x0062), __byte_perm(f[2], f[3], 0x0062), 0x5410);
       }
 #pragma unroll
-      for (int g = 0; g < N / 16; ++g)
-        *reinterpret_cast<uint4 *>(sm.p + g * 2048 + tid * 16) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+      for (int g = 0; g < kWords / 4; ++g)  // 16 columns of the key: a whole plane of the group where R is 16
+        *reinterpret_cast<uint4 *>(sm.p + (g * Sh::kGroups + wg) * 2048 + col * 16) =
+            make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
       fence_proxy_async();
       tc_fence_before();
       __syncwarp();
@@ -519,53 +535,56 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
     }
     tc_fence_before();
     // sums over the keys
-    sm.lsum[warp][reduce_index<NR>(lane)] = warp_reduce_scatter<NR>(l);
+    sm.lsum[warp & 3][wg * R + reduce_index<R>(lane)] = warp_reduce_scatter<R>(l);
+    if (lane < R && (warp & 3) == 0) sm.mrun[wg * R + lane] = m_run;
   }
   __syncwarp();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, Sh::kTmem);  // before the cluster waits: a CTA that waits for TMEM never waits for this one
   }
   const bool failed = sm.abort != 0;
   if (failed && tid == 0 && p.r.bad_flag) atomicMax(p.r.bad_flag, -QASR_ERR_TIMEOUT);
-
   float part_l = 0.0f;  // lane = row
-  if (warp < 4 && lane < NR)
+  if (lane < NR)
     part_l = failed ? __uint_as_float(0x7fc00000u)
                     : __fadd_rn(__fadd_rn(sm.lsum[0][lane], sm.lsum[1][lane]),
                                 __fadd_rn(sm.lsum[2][lane], sm.lsum[3][lane]));
   if (C == 1) {
-    if (warp < 4) {
-      const float inv = part_l == 0.0f ? 0.0f : __fdiv_rn(1.0f, part_l);
+    if (warp < Sh::kWarps) {
+      const float inv = part_l == 0.0f ? 0.0f : __frcp_rn(part_l);
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
+      for (int i = 0; i < R; ++i) {
+        const int r = wg * R + i;
         const float f = __shfl_sync(0xffffffffu, inv, r);
         const long long at = sm.at[r];
-        const bool mine = HPB == 1 || (tid >= HD) == (sm.hi >> r & 1);
-        if (at >= 0 && mine) p.out[at + tid] = __fmul_rn(acc[r], f);
+        const bool mine = HPB == 1 || (col >= HD) == (sm.hi >> r & 1);
+        if (at >= 0 && mine) p.out[at + col] = __fmul_rn(acc[i], f);
       }
     }
     return;
   }
 
-  // Row r is finished by CTA r % C (C is a power of two); partial states go there.
+  // Row r is finished by CTA r % C; partial states go there.
   cluster_wait_all();
   const int below = C - 1;
-  if (warp < 4) {
+  if (warp < Sh::kWarps) {
 #pragma unroll
-    for (int r = 0; r < NR; ++r)
-      if (r < rows) ta_store_remote(cluster_map(smem_u32(&sm.recv[(r & ~below) + rank][tid]), r & below), acc[r]);
+    for (int i = 0; i < R; ++i) {
+      const int r = wg * R + i;
+      if (r < rows) ta_store_remote(cluster_map(smem_u32(&sm.recv[(r & ~below) + rank][col]), r & below), acc[i]);
+    }
     if (warp == 0 && lane < rows) {
       const int e = (lane & ~below) + rank;
-      ta_store_remote(cluster_map(smem_u32(&sm.recv_m[e]), lane & below), m_run);
+      ta_store_remote(cluster_map(smem_u32(&sm.recv_m[e]), lane & below), sm.mrun[lane]);
       ta_store_remote(cluster_map(smem_u32(&sm.recv_l[e]), lane & below), part_l);
     }
   }
   __syncwarp();
   cluster_sync_all();
   // one warp per row: lane c has part c's maximum and sum, then four columns of the output
-  for (int r = rank + warp * C; r < rows; r += C * (kTaThreads / 32)) {
+  for (int r = rank + warp * C; r < rows; r += C * (Sh::kThreads / 32)) {
     const int e0 = r & ~below;
     const float mc = lane < C ? sm.recv_m[e0 + lane] : -INFINITY, lc = lane < C ? sm.recv_l[e0 + lane] : 0.0f;
     const float top = warp_max(mc);
@@ -582,7 +601,7 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
       o.z = fmaf(a.z, f, o.z);
       o.w = fmaf(a.w, f, o.w);
     }
-    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    const float inv = sum == 0.0f ? 0.0f : __frcp_rn(sum);
     const long long at = sm.at[r];
     const bool mine = HPB == 1 || (4 * lane >= HD) == (sm.hi >> r & 1);
     if (at >= 0 && mine)
@@ -592,7 +611,7 @@ __global__ void __launch_bounds__(kTaThreads, 2) tree_attention_kernel(const __g
 }
 
 template <int HD, int NR>
-static int tree_attention_launch(const TreeAttnParams &p, cudaStream_t st) {
+static int tree_attention_launch(TreeAttnParams p, cudaStream_t st) {
   constexpr int HPB = 128 / HD;
   const size_t smem = sizeof(TaSmem<NR>) + 1024;
   static bool attr_done[64] = {};
@@ -610,19 +629,21 @@ static int tree_attention_launch(const TreeAttnParams &p, cudaStream_t st) {
     if (rc) return rc;
     attr_done[dev] = true;
   }
-  const int W = HPB * (p.n_heads / p.c.n_kv_heads);
-  const long blocks = (long)ceil_div(p.c.n_kv_heads, HPB) * ceil_div((long)p.r.max_rows * W, NR);
-  if (blocks > 65535) {
+  const int heads = ceil_div(p.c.n_kv_heads, HPB);
+  const long row_blocks = ceil_div((long)p.r.max_rows * p.width, NR);
+  if (row_blocks > 65535) {
     set_error("qasr_tree_attention_int8: too many query rows per sequence (%d)", p.r.max_rows);
     return QASR_ERR_UNSUPPORTED;
   }
   // CTAs per block of rows: enough to fill two per SM, no more than the cache has tiles
-  int C = 1;
   const int tiles = ceil_div(p.c.max_seq, kTaKeys);
-  while (C < kTaMaxCluster && C < tiles && blocks * p.r.n_seqs * C < 148) C *= 2;
+  p.cshift = 0;
+  while (1 << p.cshift < kTaMaxCluster && 1 << p.cshift < tiles && (heads * row_blocks * p.r.n_seqs << p.cshift) < 148)
+    ++p.cshift;
+  const int C = 1 << p.cshift;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)C, (unsigned)blocks, (unsigned)p.r.n_seqs);
-  cfg.blockDim = dim3(kTaThreads);
+  cfg.gridDim = dim3((unsigned)(C * heads), (unsigned)row_blocks, (unsigned)p.r.n_seqs);
+  cfg.blockDim = dim3(TaShape<NR>::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -638,7 +659,7 @@ static int tree_attention_launch(const TreeAttnParams &p, cudaStream_t st) {
 
 template <int HD>
 static int tree_attention_rows(const TreeAttnParams &p, cudaStream_t st) {
-  const long rows = (long)p.r.max_rows * (128 / HD) * (p.n_heads / p.c.n_kv_heads);
+  const long rows = (long)p.r.max_rows * p.width;
   if (rows <= 4) return tree_attention_launch<HD, 4>(p, st);
   if (rows <= 8) return tree_attention_launch<HD, 8>(p, st);
   if (rows <= 16) return tree_attention_launch<HD, 16>(p, st);
@@ -706,6 +727,8 @@ extern "C" int qasr_tree_attention_int8(float *out, const float *q, const qasr_k
   p.tree_mask = tree_mask;
   p.layer = layer;
   p.n_heads = n_heads;
+  p.group = n_heads / cache->n_kv_heads;
+  p.width = p.group * (128 / cache->head_dim);
   p.scale = scale;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return cache->head_dim == 128 ? tree_attention_rows<128>(p, st) : tree_attention_rows<64>(p, st);
