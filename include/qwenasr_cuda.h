@@ -287,13 +287,15 @@ typedef struct {
  * device arrays, read when the kernel runs, so a captured call follows their
  * contents.  n_rows: rows of the packed buffers; those from
  * row_starts[n_seqs] on are left as they are.  max_rows: at least the rows of
- * the longest sequence (it sizes the launch).  A sequence whose entries do
+ * the longest sequence (it sizes the launch).  max_keys: how many cache rows
+ * the longest sequence may have, if the host knows (0: max_seq); attention
+ * splits its work by it, results do not depend on it.  A sequence whose entries do
  * not fit (rows outside the packed buffers or the cache, more than max_rows
  * rows, a slot outside the cache) is left out, its outputs unwritten, and sets
  * *bad_flag (device, may be NULL; never cleared) to 1. */
 typedef struct {
   const int32_t *row_starts, *positions, *slots;
-  int n_seqs, n_rows, max_rows;
+  int n_seqs, n_rows, max_rows, max_keys;
   int32_t *bad_flag;
 } qasr_kv_rows;
 

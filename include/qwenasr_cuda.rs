@@ -118,7 +118,7 @@ pub struct QasrKvInt8 {
 #[derive(Clone, Copy)]
 pub struct QasrKvRows {
     pub row_starts: *const i32, pub positions: *const i32, pub slots: *const i32,
-    pub n_seqs: c_int, pub n_rows: c_int, pub max_rows: c_int,
+    pub n_seqs: c_int, pub n_rows: c_int, pub max_rows: c_int, pub max_keys: c_int,
     pub bad_flag: *mut i32,
 }
 

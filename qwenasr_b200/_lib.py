@@ -46,7 +46,7 @@ class KvInt8(C.Structure):
 
 class KvRows(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("row_starts", "positions", "slots")] + \
-               [(n, C.c_int) for n in ("n_seqs", "n_rows", "max_rows")] + [("bad_flag", C.c_void_p)]
+               [(n, C.c_int) for n in ("n_seqs", "n_rows", "max_rows", "max_keys")] + [("bad_flag", C.c_void_p)]
 
 
 class PickRules(C.Structure):

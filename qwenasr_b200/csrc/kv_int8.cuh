@@ -26,6 +26,7 @@ QASR_DEV KvSeq kv_seq(const qasr_kv_rows &r, const qasr_kv_int8 &c, int m) {
   s.ok = s.row0 >= 0 && n >= 0 && end <= r.n_rows && n <= r.max_rows && s.pos >= 0 && s.pos + n <= c.max_seq &&
          s.slot >= 0 && s.slot < c.n_slots;
   s.n = s.ok ? (int)n : 0;
+  if (!s.ok) s.row0 = s.pos = s.slot = 0;
   return s;
 }
 

@@ -13,9 +13,10 @@
 //    digits, as in the INT8 projections.  S^T [keys x 3 digit planes of the
 //    rows] = K codes [128 keys x 128] * digits^T; the rounding of q is half a
 //    step of 2^-22 of the row's largest magnitude.
-//  * a weight e^(S - tile maximum) * vs_j / (tile's largest vs) lies in [0, 1];
-//    2^23 - 1 of it, rounded, are three unsigned digits (the low bytes of the
-//    float 2^23 + that), off by at most 2^-24 of the largest weight of the
+//  * a weight e^(S - tile maximum) * vs_j / 2^k, 2^k above the tile's largest
+//    vs, lies in [0, 1); 2^23 times it, rounded, are three unsigned digits (the
+//    low bytes of the float 2^23 + that), off by at most 2^-23 of the largest
+//    weight and value scale of the
 //    tile, below the f32 rounding of a sum over it.  O^T [128 values x digit
 //    planes] = V codes^T * digits, with V read as it lies (M-major) and the
 //    digits written by the thread that owns the key (N-major): nothing is
@@ -98,7 +99,6 @@ QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][1
 constexpr int kTaKeys = 128;             // keys of a tile: TMEM lanes of S^T
 constexpr int kTaTile = kTaKeys * 128;   // bytes of a K (or V) tile
 constexpr int kTaMaxCluster = 16;
-constexpr float kTaOne = 8388607.0f;     // a weight of 1
 constexpr float kTaMagic = 8388608.0f;   // 2^23: its low three bytes are zero
 
 // Rows of a block: NR query rows, their digit planes side by side (plane d at
@@ -108,7 +108,7 @@ struct TaShape {
   static_assert(NR == 4 || NR == 8 || NR == 16 || NR == 32, "rows of a block");
   static constexpr int kN = NR == 4 ? 16 : NR == 8 ? 32 : 3 * NR;
   static constexpr int kTmem = NR == 32 ? 256 : NR == 16 ? 128 : NR == 8 ? 64 : 32;  // S and O, a power of two
-  static constexpr int kStages = NR <= 8 ? 3 : 2;  // K and V tiles in flight
+  static constexpr int kStages = NR == 4 ? 3 : 2;  // K and V tiles in flight
   static constexpr int kGroups = NR == 32 ? 2 : 1;  // softmax warpgroups: each owns R rows of every tile
   static constexpr int kR = NR / kGroups;
   static constexpr int kChunk = kGroups > 1 ? 8 : kR;  // rows per TMEM load: eight spill less at 96 registers
@@ -139,8 +139,7 @@ struct TaSmem {
   static constexpr int kRecv = NR < kTaMaxCluster ? kTaMaxCluster : NR;
   float recv[kRecv][128], recv_m[kRecv], recv_l[kRecv];
   float4 rowc[2][Sh::kWarps][Sh::kR];  // per tile (two in flight) and warp: tile maximum, factors of the new and old sums, of O
-  float wmax[2][Sh::kWarps][Sh::kR];  // per tile and warp: row maxima
-  float wvs[2][Sh::kWarps][2];        // ... and largest value scales
+  float wmax[2][Sh::kWarps][Sh::kR + 2];  // per tile and warp: row maxima, then the largest value scales
   float qf[NR];           // 2^(E-22) * scale * log2(e)
   float lsum[4][NR], mrun[NR];
   uint32_t mask[2][NR];
@@ -264,7 +263,8 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
   }
   const bool tree = p.tree_mask != nullptr;
   const int len = s.pos + (tree ? s.n : (v0 + rows - 1) / W + 1);  // keys any row may see
-  const unsigned tiles = (unsigned)(len + kTaKeys - 1) / kTaKeys;  // < 2^25: times a rank still fits
+  const unsigned tiles = (unsigned)(len + kTaKeys - 1) / kTaKeys;
+  // below 2^25 tiles: times a rank still fits
   const int i0 = (int)(tiles * rank >> p.cshift), n = (int)(tiles * (rank + 1) >> p.cshift) - i0;
   if (C > 1) cluster_arrive_all();  // waited for before the first remote store: every CTA has started
 
@@ -344,14 +344,7 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       x4[k] = a >= 0 && b >= b0 && b < b0 + HD ? *reinterpret_cast<const float4 *>(p.q + a + b)
                                                : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (warp == 0 && lane < NR) {
-      const uint64_t mask = t >= 0 && tree ? p.tree_mask[s.row0 + t] : 0;
-      sm.mask[0][lane] = (uint32_t)mask;
-      sm.mask[1][lane] = (uint32_t)(mask >> 32);
-      sm.tok[lane] = t;
-      sm.at[lane] = at;
-      if (lane == 0) sm.hi = hi;
-    }
+    const uint64_t mask = warp == 0 && t >= 0 && tree ? p.tree_mask[s.row0 + t] : 0;
 #pragma unroll
     for (int k = 0; k < kQ; ++k) {
       const float4 x = x4[k];
@@ -368,6 +361,13 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         sm.qf[r] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : f;
       }
     }
+    if (warp == 0 && lane < NR) {
+      sm.mask[0][lane] = (uint32_t)mask;
+      sm.mask[1][lane] = (uint32_t)(mask >> 32);
+      sm.tok[lane] = t;
+      sm.at[lane] = at;
+      if (lane == 0) sm.hi = hi;
+    }
     for (int b = 3 * NR * 128 + 4 * tid; b < Sh::kQBytes; b += 512) *reinterpret_cast<uint32_t *>(sm.q + b) = 0;
     fence_proxy_async();
     named_bar(1, 32 * Sh::kWarps);
@@ -376,17 +376,21 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
     const uint32_t my_hi = hi >> (wg * R);  // bit r: the group's row r is of the pair's second head
     const int *tok = sm.tok + wg * R;
     const float *qf = sm.qf + wg * R;
-    const size_t srow = kv_row(p.c, s.slot, p.layer, 0);
     float nks[HPB], nvs[HPB];  // scales of this thread's key of the next tile
-    auto load_scales = [&](int i) {
-      const int j = (i0 + i) * kTaKeys + col;
+    int next = i0 * kTaKeys + col;
+    const size_t srow = (kv_row(p.c, s.slot, p.layer, 0) + next) * p.c.n_kv_heads + hb * HPB;
+    const float *ksp = p.c.k_scales + srow, *vsp = p.c.v_scales + srow;
+    const bool two = hb * HPB + 1 < p.c.n_kv_heads;
+    auto load_scales = [&](bool more) {
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
-        const bool in = i < n && j < len && hb * HPB + u < p.c.n_kv_heads;
-        const size_t at = (srow + j) * p.c.n_kv_heads + hb * HPB + u;
-        nks[u] = in ? __ldg(p.c.k_scales + at) : 0.0f;
-        nvs[u] = in ? __ldg(p.c.v_scales + at) : 0.0f;
+        const bool in = more && next < len && (u == 0 || two);
+        nks[u] = in ? __ldg(ksp + u) : 0.0f;
+        nvs[u] = in ? __ldg(vsp + u) : 0.0f;
       }
+      next += kTaKeys;
+      ksp += (size_t)kTaKeys * p.c.n_kv_heads;
+      vsp += (size_t)kTaKeys * p.c.n_kv_heads;
     };
     // acc = acc * old + O * coef for the tile whose constants are in rowc[b]
     auto fold = [&](int b) {
@@ -404,13 +408,13 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
     };
     // After a timeout (sm.abort) every wait returns at once and the loop runs on: a group's warps must meet at
     // the same number of barriers.  The results are thrown away.
-    load_scales(0);
+    load_scales(n > 0);
     for (int i = 0; i < n; ++i) {
       const int buf = i & 1, j = (i0 + i) * kTaKeys + col;
       float ks[HPB], vs[HPB];
 #pragma unroll
       for (int u = 0; u < HPB; ++u) ks[u] = nks[u], vs[u] = nvs[u];
-      load_scales(i + 1);
+      load_scales(i + 1 < n);
       ta_wait(sm, &sm.sfull, (unsigned)(i & 1));
       __syncwarp();
       tc_fence_after();
@@ -433,52 +437,54 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       const int place = j - s.pos;  // >= 0: the row of one of the sequence's own tokens
       if ((i0 + i + 1) * kTaKeys > s.pos) {
         if (tree) {
-          const uint32_t *mask = sm.mask[place >> 5 & 1] + wg * R;
-          const bool in = place < s.n;
+          const uint32_t *seen = sm.mask[place >> 5 & 1] + wg * R;
+          const uint32_t past = place < 0, own = place < s.n;  // bits: visible anyway, in the tree at all
           const int bit = place & 31;
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (place >= 0 && !(in && mask[r] >> bit & 1)) x[r] = -INFINITY;
+          for (int r = 0; r < R; ++r) x[r] = (past | (seen[r] >> bit & own)) ? x[r] : -INFINITY;
         } else {
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (place > tok[r] && place >= 0) x[r] = -INFINITY;
+          for (int r = 0; r < R; ++r) x[r] = place <= tok[r] ? x[r] : -INFINITY;
         }
       }
-      // a value scale that is no finite number >= 0 counts as NaN, for the rows that see it
+      // a value scale that is no number in [0, 2^125) counts as NaN, for the rows that see it
       bool odd[HPB];
-#pragma unroll
-      for (int u = 0; u < HPB; ++u) {
-        odd[u] = !(vs[u] >= 0.0f && vs[u] < INFINITY);
-        if (odd[u]) vs[u] = 0.0f;
-        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vs[u])));
-        if (lane == 0) sm.wvs[buf][warp][u] = top;
-      }
-      float mine = -INFINITY;
+      float mine = -INFINITY;  // lane r: the warp's maximum of row r; lanes R, R + 1: of the value scales
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float t = ta_warp_max(x[r]);
         if (lane == r) mine = t;
       }
-      if (lane < R) sm.wmax[buf][warp][lane] = mine;
-      named_bar(2 + wg, 128);
-      const int w0 = 4 * wg;  // the group's warps
-      float vmax[HPB];
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
-        vmax[u] = fmaxf(fmaxf(sm.wvs[buf][w0][u], sm.wvs[buf][w0 + 1][u]),
-                        fmaxf(sm.wvs[buf][w0 + 2][u], sm.wvs[buf][w0 + 3][u]));
-        vs[u] = vmax[u] > 0.0f ? __fdiv_rn(vs[u], vmax[u]) : 0.0f;
+        odd[u] = !(vs[u] >= 0.0f && vs[u] < 4.2535296e37f);
+        if (odd[u]) vs[u] = 0.0f;
+        const float t = ta_warp_max(vs[u]);
+        if (lane == R + u) mine = t;
+      }
+      if (lane < R + HPB) sm.wmax[buf][warp][lane] = mine;
+      named_bar(2 + wg, 128);
+      const int w0 = 4 * wg;  // the group's warps
+      auto over_warps = [&](int e) {
+        return fmaxf(fmaxf(sm.wmax[buf][w0][e], sm.wmax[buf][w0 + 1][e]),
+                     fmaxf(sm.wmax[buf][w0 + 2][e], sm.wmax[buf][w0 + 3][e]));
+      };
+      // Value scales relative to a power of two 2^k above the tile's largest: a weight e^(S - max) * vs * 2^-k is
+      // below 1 and nothing but its last rounding, to 23 bits, is lost.
+      float step[HPB];  // 2^(k-23): what a weight's integer counts
+#pragma unroll
+      for (int u = 0; u < HPB; ++u) {
+        const uint32_t e = (__float_as_uint(over_warps(R + u)) >> 23) + 1;  // 2^(e - 127): 1 .. 252
+        step[u] = __uint_as_float(max((int)e - 23, 1) << 23);
+        vs[u] = __fmul_rn(vs[u], __uint_as_float((254 - max((int)e - 23, 1)) << 23));
       }
       if (lane < R) {
-        const float t = fmaxf(fmaxf(sm.wmax[buf][w0][lane], sm.wmax[buf][w0 + 1][lane]),
-                              fmaxf(sm.wmax[buf][w0 + 2][lane], sm.wmax[buf][w0 + 3][lane]));
+        const float t = over_warps(lane);
         const float top = fmaxf(m_run, t), base = top == -INFINITY ? 0.0f : top;
         const float f = t == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(t, base));
         const float old = m_run == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(m_run, base));
-        const float vm = HPB == 2 && (my_hi >> lane & 1) ? vmax[HPB - 1] : vmax[0];
-        sm.rowc[buf][warp][lane] =
-            make_float4(t == -INFINITY ? 0.0f : t, f, old, __fmul_rn(f, __fmul_rn(vm, 1.0f / kTaOne)));
+        sm.rowc[buf][warp][lane] = make_float4(t == -INFINITY ? 0.0f : t, f, old,
+                                               __fmul_rn(f, HPB == 2 && (my_hi >> lane & 1) ? step[HPB - 1] : step[0]));
         m_run = top;
       }
       __syncwarp();
@@ -510,7 +516,7 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
           const float pr = ta_ex2(__fsub_rn(x[r], c.x));
           l[r] = fmaf(l[r], c.z, __fmul_rn(pr, c.y));
           const float v = HPB == 2 && (my_hi >> r & 1) ? vs[HPB - 1] : vs[0];
-          f[e] = __float_as_uint(fmaf(__fmul_rn(pr, v), kTaOne, kTaMagic));
+          f[e] = __float_as_uint(fmaf(pr, v, kTaMagic));
         }
         // bytes 0, 1 and 2 of the four rows
         const uint32_t a = __byte_perm(f[0], f[1], 0x5140), b = __byte_perm(f[2], f[3], 0x5140);
@@ -635,11 +641,17 @@ static int tree_attention_launch(TreeAttnParams p, cudaStream_t st) {
     set_error("qasr_tree_attention_int8: too many query rows per sequence (%d)", p.r.max_rows);
     return QASR_ERR_UNSUPPORTED;
   }
-  // CTAs per block of rows: enough to fill two per SM, no more than the cache has tiles
-  const int tiles = ceil_div(p.c.max_seq, kTaKeys);
+  // CTAs per block of rows.  A CTA costs 3 to 4 us beside its tiles, so no more than 256 of them in all (32
+  // blocks over 1000 rows: 5.8 us with 8 each, 14.5 with 16; 64 blocks 6.6 with 4, 11.1 with 8), but up to 512
+  // where long histories (32 tiles) may differ in length and the longest would set the time: 256 blocks over 250 ..
+  // 8000 rows take 48 us with two each and 61 with one (all 8000: 88 and 82).  Sixteen of a cluster find room on
+  // few SMs of a GPC at a time: only for 8 blocks (2000 rows: 5.4 us, 5.8 with 8; 16 blocks 9.6 and 5.3).
+  const int keys = p.r.max_keys > 0 ? std::min(p.r.max_keys, p.c.max_seq) : p.c.max_seq;
+  const int tiles = ceil_div(keys, kTaKeys);
+  const long blocks = (long)heads * row_blocks * p.r.n_seqs;
+  const int most = blocks <= 8 && tiles >= 16 ? 16 : 8;
   p.cshift = 0;
-  while (1 << p.cshift < kTaMaxCluster && 1 << p.cshift < tiles && (heads * row_blocks * p.r.n_seqs << p.cshift) < 148)
-    ++p.cshift;
+  for (int C = 2; C <= most && C < 2 * tiles && blocks * C <= (C <= 4 && tiles >= 32 ? 512 : 256); C *= 2) ++p.cshift;
   const int C = 1 << p.cshift;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(C * heads), (unsigned)row_blocks, (unsigned)p.r.n_seqs);

@@ -61,10 +61,12 @@ class KvRows:
     of slot slots[m] (slots None: slot m).  int32 device tensors, read when the
     kernels run: they may be changed in place between calls or graph replays.
     n_rows: rows of the packed buffers; max_rows: a bound on one sequence's
-    rows; bad_flag: int32 [1], set when a sequence does not fit."""
+    rows; max_keys: a bound on one sequence's cache rows, by which attention
+    splits its work (0: the cache's max_seq); bad_flag: int32 [1], set when a
+    sequence does not fit."""
 
     def __init__(self, row_starts: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor | None = None, *,
-                 n_rows: int, max_rows: int, bad_flag: torch.Tensor | None = None):
+                 n_rows: int, max_rows: int, max_keys: int = 0, bad_flag: torch.Tensor | None = None):
         n = row_starts.numel() - 1 if isinstance(row_starts, torch.Tensor) else -1
         if n < 0:
             raise ValueError("row_starts must be a tensor of n_seqs + 1 entries")
@@ -76,6 +78,6 @@ class KvRows:
         if bad_flag is not None:
             _tensor(bad_flag, torch.int32, self.device, "bad_flag", 1)
         self.row_starts, self.positions, self.slots, self.bad_flag = row_starts, positions, slots, bad_flag
-        self.n_seqs, self.n_rows, self.max_rows = n, int(n_rows), int(max_rows)
+        self.n_seqs, self.n_rows, self.max_rows, self.max_keys = n, int(n_rows), int(max_rows), int(max_keys)
         self.c = _lib.KvRows(row_starts.data_ptr(), positions.data_ptr(), None if slots is None else slots.data_ptr(),
-                             n, self.n_rows, self.max_rows, None if bad_flag is None else bad_flag.data_ptr())
+                             n, self.n_rows, self.max_rows, self.max_keys, None if bad_flag is None else bad_flag.data_ptr())

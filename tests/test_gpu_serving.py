@@ -7,10 +7,11 @@ and are compared bit for bit.  Attention: with
   dS  = scale * max|q| * 2^-22 * max_j sum_d |k_jd|  (q to 23 bits of its row's
         maximum, half a step)  + 8 * 2^-24 * max|S|  (the f32 steps from the sum
         to the exponent's argument),
-a weight is off by a factor e^(2 dS) * (1 + 2^-21) (the exponential) and by 2^-24 of
-the largest weight of its 128-key tile (23-bit weights); every f32 sum of n
-terms of one sign by n * 2^-24.  All of it multiplies values of at most vmax,
-so |out - exact| <= vmax * (4 dS + 2^-20 + 128 * 2^-24 + (n / 128 + 128) * 2^-24).
+a weight is off by a factor e^(2 dS) * (1 + 2^-21) (the exponential) and by 2^-23 of
+the largest weight of its 128-key tile (half a step of 23 bits below a power of
+two that is at most twice the largest); every f32 sum of n terms of one sign by
+n * 2^-24.  All of it multiplies values of at most vmax, so
+|out - exact| <= vmax * (4 dS + 2^-20 + 128 * 2^-23 + (n / 128 + 128) * 2^-24).
 """
 import math
 
@@ -262,7 +263,7 @@ def attend_exact(c, layer, q, counts, positions, slots, masks, n_heads, scale):
                     w = np.exp(s - s.max())
                     o = w @ v[see] / w.sum()
                     ds = scale * np.abs(x).max() * 2.0 ** -22 * np.abs(k[see]).sum(1).max() + 2.0 ** -21 * np.abs(s).max()
-                    tol = 4 * ds + 2.0 ** -20 + 2.0 ** -17 + (len(s) / 128 + 128) * 2.0 ** -24
+                    tol = 4 * ds + 2.0 ** -20 + 2.0 ** -16 + (len(s) / 128 + 128) * 2.0 ** -24
                     bar[r0 + t] = max(bar[r0 + t, 0], np.abs(v[see]).max() * tol)
                 out[r0 + t, h * hd:(h + 1) * hd] = o
     return out, bar
@@ -421,7 +422,7 @@ def test_long_cache_offsets():
         w = np.exp(s - mx)
         ref = w @ (vq[:, cut].astype(np.float64) * vs[:, h, None]) / (w.sum() + (max_seq - 300) * np.exp(-mx))
         ds = 0.0884 * np.abs(q[0, cut]).max() * 2.0 ** -22 * np.abs(k).sum(1).max() + 2.0 ** -21 * np.abs(s).max()
-        tol = 4 * ds + 2.0 ** -20 + 2.0 ** -17 + (max_seq / 128 + 128) * 2.0 ** -24
+        tol = 4 * ds + 2.0 ** -20 + 2.0 ** -16 + (max_seq / 128 + 128) * 2.0 ** -24
         assert (np.abs(got[h] - ref) <= np.abs(y).max() * tol).all()
 
 

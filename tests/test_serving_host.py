@@ -27,7 +27,7 @@ def cache(**kw):
 
 
 def rows(**kw):
-    d = dict(row_starts=256, positions=256, slots=None, n_seqs=2, n_rows=4, max_rows=2, bad_flag=None)
+    d = dict(row_starts=256, positions=256, slots=None, n_seqs=2, n_rows=4, max_rows=2, max_keys=0, bad_flag=None)
     d.update(kw)
     return C.byref(_lib.KvRows(*d.values()))
 
