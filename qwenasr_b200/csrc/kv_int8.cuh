@@ -15,31 +15,48 @@ struct KvSeq {
   bool ok;
 };
 
-QASR_DEV KvSeq kv_seq(const qasr_kv_rows &r, const qasr_kv_int8 &c, int m) {
-  KvSeq s;
-  s.row0 = r.row_starts[m];
-  const int end = r.row_starts[m + 1];
-  s.pos = r.positions[m];
-  s.slot = r.slots ? r.slots[m] : m;
-  // in 64 bits: the entries may be anything
-  const long long n = (long long)end - s.row0;
-  s.ok = s.row0 >= 0 && n >= 0 && end <= r.n_rows && n <= r.max_rows && s.pos >= 0 && s.pos + n <= c.max_seq &&
-         s.slot >= 0 && s.slot < c.n_slots;
-  s.n = s.ok ? (int)n : 0;
-  if (!s.ok) s.row0 = s.pos = s.slot = 0;
+// The raw entries of sequence m, checked.
+QASR_DEV KvSeq kv_seq_checked(const qasr_kv_rows &r, const qasr_kv_int8 &c, int start, int end, int pos, int slot) {
+  KvSeq s{start, 0, pos, slot, false};
+  const long long n = (long long)end - start;  // in 64 bits: the entries may be anything
+  s.ok = start >= 0 && n >= 0 && end <= r.n_rows && n <= r.max_rows && pos >= 0 && pos + n <= c.max_seq && slot >= 0 &&
+         slot < c.n_slots;
+  if (s.ok)
+    s.n = (int)n;
+  else
+    s.row0 = s.pos = s.slot = 0;
   return s;
 }
 
-// Whole warp: the sequence that owns packed row `row`, or -1.  Counts the
-// starts at or below the row, 32 at a time; entries in disorder give a
-// sequence that does not hold the row, which kv_seq's caller checks.
-QASR_DEV int kv_seq_of_row(const qasr_kv_rows &r, int row, int lane) {
-  int m = -1;
+QASR_DEV KvSeq kv_seq(const qasr_kv_rows &r, const qasr_kv_int8 &c, int m) {
+  return kv_seq_checked(r, c, r.row_starts[m], r.row_starts[m + 1], r.positions[m], r.slots ? r.slots[m] : m);
+}
+
+// Whole warp: where packed row `row` stands in the cache; ok = false for a row
+// behind the last sequence or of one that does not fit.  The owner is the last
+// sequence that starts at or below the row, found 32 at a time; its entries
+// come along in the same round of loads.  Starts in disorder give a sequence
+// that does not hold the row.
+struct KvPlace {
+  bool ok;
+  int slot, pos;
+};
+QASR_DEV KvPlace kv_place(const qasr_kv_rows &r, const qasr_kv_int8 &c, int row, int lane) {
+  KvPlace at{false, 0, 0};
   for (int base = 0; base < r.n_seqs; base += 32) {
     const int i = base + lane;
-    m += __popc(__ballot_sync(0xffffffffu, i < r.n_seqs && r.row_starts[i] <= row));
+    const bool in = i < r.n_seqs;
+    const int start = in ? r.row_starts[i] : 0, end = in ? r.row_starts[i + 1] : 0, pos = in ? r.positions[i] : 0;
+    const int slot = in && r.slots ? r.slots[i] : i;
+    const int below = __popc(__ballot_sync(0xffffffffu, in && start <= row));
+    if (below == 0) break;
+    const int own = below - 1;
+    const KvSeq s = kv_seq_checked(r, c, __shfl_sync(0xffffffffu, start, own), __shfl_sync(0xffffffffu, end, own),
+                                   __shfl_sync(0xffffffffu, pos, own), __shfl_sync(0xffffffffu, slot, own));
+    at = KvPlace{row >= s.row0 && row - s.row0 < s.n, s.slot, s.pos + (row - s.row0)};
+    if (below < 32) break;
   }
-  return m;
+  return at;
 }
 
 // One warp of a launch: every sequence's entries, *bad_flag if one does not fit.

@@ -64,6 +64,11 @@ def test_bad_rows(lib, kw):
         assert name in _lib.last_error()
 
 
+def test_too_many_rows(lib):
+    for name, rc in calls(lib, cache(), rows(n_rows=1 << 29)):
+        assert rc == _lib.QASR_ERR_UNSUPPORTED, name
+
+
 @pytest.mark.parametrize("layer", [-1, 3])
 def test_bad_layer(lib, layer):
     assert lib.qasr_kv_append_int8(cache(), layer, rows(), P, P, None, 4, None) == _lib.QASR_ERR_INVALID
