@@ -13,14 +13,13 @@
 //    digits, as in the INT8 projections.  S^T [keys x 3 digit planes of the
 //    rows] = K codes [128 keys x 128] * digits^T; the rounding of q is half a
 //    step of 2^-22 of the row's largest magnitude.
-//  * a weight e^(S - tile maximum) * vs_j / 2^k, 2^k above the tile's largest
-//    vs, lies in [0, 1); 2^23 times it, rounded, are three unsigned digits (the
-//    low bytes of the float 2^23 + that), off by at most 2^-23 of the largest
-//    weight and value scale of the
-//    tile, below the f32 rounding of a sum over it.  O^T [128 values x digit
-//    planes] = V codes^T * digits, with V read as it lies (M-major) and the
-//    digits written by the thread that owns the key (N-major): nothing is
-//    transposed or converted on the way.
+//  * a weight e^(S - tile maximum) * vs_j / (the tile's largest vs) lies in
+//    [0, 1]; 2^23 times it, rounded, are three unsigned digits (the low bytes of
+//    the float 2^23 + that), off by at most 2^-24 of the largest weight and
+//    value scale of the tile, below the f32 rounding of a sum over it.  O^T [128
+//    values x digit planes] = V codes^T * digits, with V read as it lies
+//    (M-major) and the digits written by the thread that owns the key (N-major):
+//    nothing is transposed or converted on the way.
 // Digit sums are recombined in f32 (one rounding below the value's own) and
 // accumulated over the tiles in f32 with the usual running maximum and sum.
 //
@@ -168,6 +167,11 @@ constexpr uint32_t ta_idesc_o(int N) {
 QASR_DEV float ta_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+QASR_DEV float ta_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 QASR_DEV float ta_warp_max(float x) {
@@ -469,14 +473,14 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         return fmaxf(fmaxf(sm.wmax[buf][w0][e], sm.wmax[buf][w0 + 1][e]),
                      fmaxf(sm.wmax[buf][w0 + 2][e], sm.wmax[buf][w0 + 3][e]));
       };
-      // Value scales relative to a power of two 2^k above the tile's largest: a weight e^(S - max) * vs * 2^-k is
-      // below 1 and nothing but its last rounding, to 23 bits, is lost.
-      float step[HPB];  // 2^(k-23): what a weight's integer counts
+      // Value scales relative to the tile's largest, times 2^23: a weight's integer is e^(S - max) * vs / largest *
+      // 2^23, its last rounding half a unit.  The reciprocal's own error scales the whole tile, by an ulp or two.
+      float step[HPB];  // what a unit counts
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
-        const uint32_t e = (__float_as_uint(over_warps(R + u)) >> 23) + 1;  // 2^(e - 127): 1 .. 252
-        step[u] = __uint_as_float(max((int)e - 23, 1) << 23);
-        vs[u] = __fmul_rn(vs[u], __uint_as_float((254 - max((int)e - 23, 1)) << 23));
+        const float t = fmaxf(over_warps(R + u), 7.888609e-31f);  // 2^-100: below it values lose bits instead
+        step[u] = __fmul_rn(t, 1.0f / kTaMagic);
+        vs[u] = __fmul_rn(vs[u], __fmul_rn(kTaMagic, ta_rcp(t)));
       }
       if (lane < R) {
         const float t = over_warps(lane);

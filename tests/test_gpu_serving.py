@@ -8,9 +8,8 @@ and are compared bit for bit.  Attention: with
         maximum, half a step)  + 8 * 2^-24 * max|S|  (the f32 steps from the sum
         to the exponent's argument),
 a weight is off by a factor e^(2 dS) * (1 + 2^-21) (the exponential) and by 2^-23 of
-the largest weight of its 128-key tile (half a step of 23 bits below a power of
-two that is at most twice the largest); every f32 sum of n terms of one sign by
-n * 2^-24.  All of it multiplies values of at most vmax, so
+the largest weight of its 128-key tile (23 bits, half a step and the largest's own
+rounding); every f32 sum of n terms of one sign by n * 2^-24.  All of it multiplies values of at most vmax, so
 |out - exact| <= vmax * (4 dS + 2^-20 + 128 * 2^-23 + (n / 128 + 128) * 2^-24).
 """
 import math
