@@ -271,30 +271,36 @@ def _need(t, dtype, dev, name, numel):
     These calls are short and a step makes several per layer, so the checks run once, without _ptr's objects."""
     if t is None:
         return None
+    try:
+        if t.get_device() == dev and t.dtype is dtype and t.numel() >= numel and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or t.get_device() != dev:
         raise ValueError(f"{name} must be a CUDA tensor on cuda:{dev}")
-    if t.dtype is not dtype or not t.is_contiguous() or t.numel() < numel:
-        _ptr(t, dtype, name, numel)  # raises with the reason
-    return t.data_ptr()
+    _ptr(t, dtype, name, numel)  # raises with the reason
 
 
-# The current stream's handle by device index, without a Stream object (several times the cost of the rest of a call).
+# Current device and stream by index, without the checks and objects of torch.cuda's own (most of a call's cost).
+_get_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _on(dev, name, *args):
     """Call an entry on device index `dev`, on that device's current stream (the last argument)."""
-    if torch.cuda.current_device() == dev:
-        _lib.call(name, *args, _raw_stream(dev))
+    if _get_device() == dev:
+        code = getattr(_lib._lib or _lib.load(), name)(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, _raw_stream(dev))
+            code = getattr(_lib._lib or _lib.load(), name)(*args, _raw_stream(dev))
+    if code != _lib.QASR_OK:
+        _lib.check(code, name)
 
 
 def _kv_args(cache, rows):
-    if rows.device != cache.device:
+    if rows.dev != cache.dev:
         raise ValueError(f"rows are on {rows.device}, the cache on {cache.device}")
-    return cache.device.index, rows.n_rows
+    return cache.dev, rows.n_rows
 
 
 def kv_append_int8(cache, layer, rows, k_new, v_new, src_rows=None):
@@ -302,9 +308,11 @@ def kv_append_int8(cache, layer, rows, k_new, v_new, src_rows=None):
     of a KvCacheInt8 at the places of `rows` (KvRows); packed row r takes source
     row src_rows[r] (int32) or r.  The f32 form is kv_append."""
     dev, n = _kv_args(cache, rows)
+    if k_new is None or v_new is None:
+        raise ValueError("k_new and v_new must be tensors")
     need = 0 if src_rows is not None else n * cache.kv_dim
     k, v = _need(k_new, f32, dev, "k_new", need), _need(v_new, f32, dev, "v_new", need)
-    _on(dev, "qasr_kv_append_int8", C.byref(cache.c), layer, C.byref(rows.c), k, v,
+    _on(dev, "qasr_kv_append_int8", cache.ref, layer, rows.ref, k, v,
         _need(src_rows, i32, dev, "src_rows", n), min(k_new.numel(), v_new.numel()) // cache.kv_dim)
 
 
@@ -312,7 +320,7 @@ def kv_read_int8(k_out, v_out, cache, layer, rows):
     """The cache rows of `rows` as f32 into k_out, v_out [n_rows, n_kv_heads * head_dim]; either may be None."""
     dev, n = _kv_args(cache, rows)
     _on(dev, "qasr_kv_read_int8", _need(k_out, f32, dev, "k_out", n * cache.kv_dim),
-        _need(v_out, f32, dev, "v_out", n * cache.kv_dim), C.byref(cache.c), layer, C.byref(rows.c))
+        _need(v_out, f32, dev, "v_out", n * cache.kv_dim), cache.ref, layer, rows.ref)
 
 
 def tree_attention_int8(out, q, cache, layer, rows, n_heads, scale, tree_mask=None):
@@ -323,8 +331,8 @@ def tree_attention_int8(out, q, cache, layer, rows, n_heads, scale, tree_mask=No
     dev, n = _kv_args(cache, rows)
     size = n * n_heads * cache.head_dim
     _on(dev, "qasr_tree_attention_int8", _need(out, f32, dev, "out", size), _need(q, f32, dev, "q", size),
-        C.byref(cache.c), layer, C.byref(rows.c), _need(tree_mask, torch.int64, dev, "tree_mask", n), n_heads,
-        C.c_float(scale))
+        cache.ref, layer, rows.ref, _need(tree_mask, torch.int64, dev, "tree_mask", n), n_heads,
+        scale)
 
 
 def logits_pick(ids_out, logits_out, logits, M, vocab, history=None, history_starts=None, repetition=None,
@@ -337,18 +345,15 @@ def logits_pick(ids_out, logits_out, logits, M, vocab, history=None, history_sta
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
     dev = logits.get_device()
-
-    def opt(t, dtype, name, numel):
-        return _need(t, dtype, dev, name, numel)
-
+    n_hist = 0 if history is None else history.numel()
     n_bias = 0 if bias_ids is None else bias_ids.numel()
-    r = _lib.PickRules(opt(history, i32, "history", 0), opt(history_starts, i32, "history_starts", M + 1),
-                       0 if history is None else history.numel(), opt(repetition, f32, "repetition", M),
-                       opt(presence, f32, "presence", M), opt(frequency, f32, "frequency", M),
-                       opt(bias_ids, i32, "bias_ids", 0), opt(bias_values, f32, "bias_values", n_bias),
-                       opt(bias_starts, i32, "bias_starts", M + 1), n_bias,
-                       opt(allow_mask, i32, "allow_mask", M * ((vocab + 31) // 32)),
-                       opt(bad_flag, i32, "bad_flag", 1))
+    r = _lib.PickRules(_need(history, i32, dev, "history", 0), _need(history_starts, i32, dev, "history_starts", M + 1),
+                       n_hist, _need(repetition, f32, dev, "repetition", M), _need(presence, f32, dev, "presence", M),
+                       _need(frequency, f32, dev, "frequency", M), _need(bias_ids, i32, dev, "bias_ids", 0),
+                       _need(bias_values, f32, dev, "bias_values", n_bias),
+                       _need(bias_starts, i32, dev, "bias_starts", M + 1), n_bias,
+                       _need(allow_mask, i32, dev, "allow_mask", M * ((vocab + 31) // 32)),
+                       _need(bad_flag, i32, dev, "bad_flag", 1))
     _on(dev, "qasr_logits_pick", _need(ids_out, i32, dev, "ids_out", M),
         _need(logits_out, f32, dev, "logits_out", M * vocab), _need(logits, f32, dev, "logits", M * vocab), C.byref(r),
         M, vocab)

@@ -46,6 +46,7 @@ class KvCacheInt8:
         self.n_kv_heads, self.head_dim = n_kv, self.kv_dim // n_kv
         self.c = _lib.KvInt8(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), self.n_slots,
                              self.n_layers, self.max_seq, n_kv, self.head_dim)
+        self.ref, self.dev = C.byref(self.c), k.get_device()
 
     @classmethod
     def zeros(cls, n_slots: int, n_layers: int, max_seq: int, n_kv_heads: int, head_dim: int, device="cuda:0"):
@@ -81,3 +82,4 @@ class KvRows:
         self.n_seqs, self.n_rows, self.max_rows, self.max_keys = n, int(n_rows), int(max_rows), int(max_keys)
         self.c = _lib.KvRows(row_starts.data_ptr(), positions.data_ptr(), None if slots is None else slots.data_ptr(),
                              n, self.n_rows, self.max_rows, self.max_keys, None if bad_flag is None else bad_flag.data_ptr())
+        self.ref, self.dev = C.byref(self.c), row_starts.get_device()
