@@ -95,6 +95,31 @@ QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][1
       : "memory");
 }
 
+// Two f32 in one register pair: rows go two at a time through the f32 steps.
+using F2 = unsigned long long;
+QASR_DEV F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+QASR_DEV float f2_lo(F2 a) { return __uint_as_float((uint32_t)a); }
+QASR_DEV float f2_hi(F2 a) { return __uint_as_float((uint32_t)(a >> 32)); }
+QASR_DEV F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+QASR_DEV F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+QASR_DEV F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 constexpr int kTaKeys = 128;             // keys of a tile: TMEM lanes of S^T
 constexpr int kTaTile = kTaKeys * 128;   // bytes of a K (or V) tile
 constexpr int kTaMaxCluster = 16;
@@ -137,9 +162,11 @@ struct TaSmem {
   // partial states pushed by the cluster: entry r / C * C + c is CTA c's of row r, one of the rows r % C = rank
   static constexpr int kRecv = NR < kTaMaxCluster ? kTaMaxCluster : NR;
   float recv[kRecv][128], recv_m[kRecv], recv_l[kRecv];
-  float4 rowc[2][Sh::kWarps][Sh::kR];  // per tile (two in flight) and warp: tile maximum, factors of the new and old sums, of O
+  // per tile (two in flight), warp and pair of rows: minus the tile maximum, the factors of the tile's sum, of the
+  // sums before it and of O
+  alignas(16) F2 rowc[2][Sh::kWarps][Sh::kR / 2][4];
   float wmax[2][Sh::kWarps][Sh::kR + 2];  // per tile and warp: row maxima, then the largest value scales
-  float qf[NR];           // 2^(E-22) * scale * log2(e)
+  alignas(16) float qf[NR];  // 2^(E-22) * scale * log2(e)
   float lsum[4][NR], mrun[NR];
   uint32_t mask[2][NR];
   int tok[NR];            // the row's token, -1 for none
@@ -272,9 +299,11 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
   const int i0 = (int)(tiles * rank >> p.cshift), n = (int)(tiles * (rank + 1) >> p.cshift) - i0;
   if (C > 1) cluster_arrive_all();  // waited for before the first remote store: every CTA has started
 
-  float acc[R], l[R], m_run = -INFINITY;  // thread = value column (acc), key (l); lane = row (m_run)
+  // thread = value column (acc2), key (l2), two rows each; lane = row (m_run)
+  F2 acc2[R / 2], l2[R / 2];
+  float m_run = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < R; ++r) acc[r] = l[r] = 0.0f;
+  for (int r = 0; r < R / 2; ++r) acc2[r] = l2[r] = 0ull;
   const int col = tid & 127, wg = warp >> 2;  // softmax warps: key / value column, first row wg * R
 
   if (warp == kTmaWarp) {
@@ -403,10 +432,12 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         uint32_t d[3][CH];
         tmem_ld_planes(my_o + c0, NR, d);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const float4 c = sm.rowc[b][warp][c0 + i];
-          const float o = fmaf((float)(int)d[2][i], 65536.0f, (float)((int)d[1][i] * 256 + (int)d[0][i]));
-          acc[c0 + i] = fmaf(acc[c0 + i], c.z, __fmul_rn(o, c.w));
+        for (int i = 0; i < CH; i += 2) {
+          const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(&sm.rowc[b][warp][(c0 + i) / 2][2]);
+          const F2 o = f2_fma(f2((float)(int)d[2][i], (float)(int)d[2][i + 1]), f2(65536.0f, 65536.0f),
+                              f2((float)((int)d[1][i] * 256 + (int)d[0][i]),
+                                 (float)((int)d[1][i + 1] * 256 + (int)d[0][i + 1])));
+          acc2[(c0 + i) / 2] = f2_fma(acc2[(c0 + i) / 2], c.x, f2_mul(o, c.y));
         }
       }
     };
@@ -428,11 +459,16 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         uint32_t d[3][CH];
         tmem_ld_planes(my_s + c0, NR, d);
 #pragma unroll
-        for (int e = 0; e < CH; ++e) {
+        for (int e = 0; e < CH; e += 2) {
           const int r = c0 + e;
-          const float k = HPB == 2 && (my_hi >> r & 1) ? ks[HPB - 1] : ks[0];
-          const float sum = fmaf((float)(int)d[0][e], 65536.0f, (float)((int)d[1][e] * 256 + (int)d[2][e]));
-          x[r] = __fmul_rn(sum, __fmul_rn(qf[r], k));
+          const F2 k = f2(HPB == 2 && (my_hi >> r & 1) ? ks[HPB - 1] : ks[0],
+                          HPB == 2 && (my_hi >> (r + 1) & 1) ? ks[HPB - 1] : ks[0]);
+          const F2 sum = f2_fma(f2((float)(int)d[0][e], (float)(int)d[0][e + 1]), f2(65536.0f, 65536.0f),
+                                f2((float)((int)d[1][e] * 256 + (int)d[2][e]),
+                                   (float)((int)d[1][e + 1] * 256 + (int)d[2][e + 1])));
+          const F2 x2 = f2_mul(sum, f2_mul(*reinterpret_cast<const F2 *>(qf + r), k));
+          x[r] = f2_lo(x2);
+          x[r + 1] = f2_hi(x2);
         }
       }
       tc_fence_before();
@@ -487,8 +523,11 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         const float top = fmaxf(m_run, t), base = top == -INFINITY ? 0.0f : top;
         const float f = t == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(t, base));
         const float old = m_run == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(m_run, base));
-        sm.rowc[buf][warp][lane] = make_float4(t == -INFINITY ? 0.0f : t, f, old,
-                                               __fmul_rn(f, HPB == 2 && (my_hi >> lane & 1) ? step[HPB - 1] : step[0]));
+        float *c = reinterpret_cast<float *>(sm.rowc[buf][warp][lane / 2]) + lane % 2;
+        c[0] = t == -INFINITY ? 0.0f : -t;
+        c[2] = f;
+        c[4] = old;
+        c[6] = __fmul_rn(f, HPB == 2 && (my_hi >> lane & 1) ? step[HPB - 1] : step[0]);
         m_run = top;
       }
       __syncwarp();
@@ -498,7 +537,7 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
           if (x[r] != -INFINITY && (HPB == 2 && (my_hi >> r & 1) ? odd[HPB - 1] : odd[0]))
-            l[r] = __uint_as_float(0x7fc00000u);
+            l2[r / 2] |= 0x7fc00000ull << (r % 2 * 32);  // a quiet NaN whatever it was
       }
       if (i > 0) {  // the previous tile's O; its digits in sm.p are free after it
         ta_wait(sm, &sm.ofull, (unsigned)((i - 1) & 1));
@@ -514,13 +553,18 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       for (int r0 = 0; r0 < R; r0 += 4) {
         uint32_t f[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; e += 2) {
           const int r = r0 + e;
-          const float4 c = sm.rowc[buf][warp][r];
-          const float pr = ta_ex2(__fsub_rn(x[r], c.x));
-          l[r] = fmaf(l[r], c.z, __fmul_rn(pr, c.y));
-          const float v = HPB == 2 && (my_hi >> r & 1) ? vs[HPB - 1] : vs[0];
-          f[e] = __float_as_uint(fmaf(pr, v, kTaMagic));
+          const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(&sm.rowc[buf][warp][r / 2][0]);
+          const F2 old = sm.rowc[buf][warp][r / 2][2];
+          const F2 y = f2_add(f2(x[r], x[r + 1]), c.x);
+          const F2 pr = f2(ta_ex2(f2_lo(y)), ta_ex2(f2_hi(y)));
+          l2[r / 2] = f2_fma(l2[r / 2], old, f2_mul(pr, c.y));
+          const F2 v = f2(HPB == 2 && (my_hi >> r & 1) ? vs[HPB - 1] : vs[0],
+                          HPB == 2 && (my_hi >> (r + 1) & 1) ? vs[HPB - 1] : vs[0]);
+          const F2 w2 = f2_fma(pr, v, f2(kTaMagic, kTaMagic));
+          f[e] = (uint32_t)w2;
+          f[e + 1] = (uint32_t)(w2 >> 32);
         }
         // bytes 0, 1 and 2 of the four rows
         const uint32_t a = __byte_perm(f[0], f[1], 0x5140), b = __byte_perm(f[2], f[3], 0x5140);
@@ -545,6 +589,9 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
     }
     tc_fence_before();
     // sums over the keys
+    float l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) l[r] = r % 2 ? f2_hi(l2[r / 2]) : f2_lo(l2[r / 2]);
     sm.lsum[warp & 3][wg * R + reduce_index<R>(lane)] = warp_reduce_scatter<R>(l);
     if (lane < R && (warp & 3) == 0) sm.mrun[wg * R + lane] = m_run;
   }
@@ -570,7 +617,7 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         const float f = __shfl_sync(0xffffffffu, inv, r);
         const long long at = sm.at[r];
         const bool mine = HPB == 1 || (col >= HD) == (sm.hi >> r & 1);
-        if (at >= 0 && mine) p.out[at + col] = __fmul_rn(acc[i], f);
+        if (at >= 0 && mine) p.out[at + col] = __fmul_rn(i % 2 ? f2_hi(acc2[i / 2]) : f2_lo(acc2[i / 2]), f);
       }
     }
     return;
@@ -583,7 +630,9 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int r = wg * R + i;
-      if (r < rows) ta_store_remote(cluster_map(smem_u32(&sm.recv[(r & ~below) + rank][col]), r & below), acc[i]);
+      if (r < rows)
+        ta_store_remote(cluster_map(smem_u32(&sm.recv[(r & ~below) + rank][col]), r & below),
+                        i % 2 ? f2_hi(acc2[i / 2]) : f2_lo(acc2[i / 2]));
     }
     if (warp == 0 && lane < rows) {
       const int e = (lane & ~below) + rank;
