@@ -165,7 +165,7 @@ struct TaSmem {
   // per tile (two in flight), warp and pair of rows: minus the tile maximum, the factors of the tile's sum, of the
   // sums before it and of O
   alignas(16) F2 rowc[2][Sh::kWarps][Sh::kR / 2][4];
-  float wmax[2][Sh::kWarps][Sh::kR + 2];  // per tile and warp: row maxima, then the largest value scales
+  alignas(16) float wmax[2][Sh::kWarps][Sh::kR + 4];  // per tile and warp: row maxima, then the largest value scales
   alignas(16) float qf[NR];  // 2^(E-22) * scale * log2(e)
   float lsum[4][NR], mrun[NR];
   uint32_t mask[2][NR];
@@ -247,7 +247,8 @@ QASR_DEV void ta_put_digits(unsigned char *q, int r, int b, float4 v, float qm) 
 }
 
 // HD: head_dim; HPB = 128 / HD kv heads share a tile.  Grid: (C x head blocks,
-// row blocks, sequences), clusters of C along x.
+// row blocks, sequences), clusters of C along x; the last rows, which see the
+// most keys, come first.
 template <int HD, int NR>
 __global__ void __launch_bounds__(TaShape<NR>::kThreads, 2)
 tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
@@ -285,7 +286,7 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
   pdl_wait();
 
   const KvSeq s = kv_seq(p.r, p.c, m);
-  const int v0 = blockIdx.y * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
+  const int v0 = (int)(gridDim.y - 1 - blockIdx.y) * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
   const bool first = blockIdx.x == 0 && blockIdx.y == 0 && m == 0;
   if (rows <= 0) {  // the whole cluster
     if (first && warp == 0) kv_flag_bad(p.r, p.c, lane);
@@ -489,20 +490,22 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       }
       // a value scale that is no number in [0, 2^125) counts as NaN, for the rows that see it
       bool odd[HPB];
-      float mine = -INFINITY;  // lane r: the warp's maximum of row r; lanes R, R + 1: of the value scales
+      float top[R + 4];  // the warp's row maxima, then those of the value scales
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float t = ta_warp_max(x[r]);
-        if (lane == r) mine = t;
-      }
+      for (int r = 0; r < R; ++r) top[r] = ta_warp_max(x[r]);
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
         odd[u] = !(vs[u] >= 0.0f && vs[u] < 4.2535296e37f);
         if (odd[u]) vs[u] = 0.0f;
-        const float t = ta_warp_max(vs[u]);
-        if (lane == R + u) mine = t;
+        top[R + u] = ta_warp_max(vs[u]);
       }
-      if (lane < R + HPB) sm.wmax[buf][warp][lane] = mine;
+#pragma unroll
+      for (int u = HPB; u < 4; ++u) top[R + u] = 0.0f;
+      if (lane == 0) {
+#pragma unroll
+        for (int r = 0; r < R + 4; r += 4)
+          *reinterpret_cast<float4 *>(&sm.wmax[buf][warp][r]) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
+      }
       named_bar(2 + wg, 128);
       const int w0 = 4 * wg;  // the group's warps
       auto over_warps = [&](int e) {
