@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) logits_pick_kernel(const Pick
   const uint32_t *mask = MASK ? r.allow_mask + (size_t)m * ((V + 31) / 32) : nullptr;
   const int c0 = (int)min((long)rank * p.chunk, (long)V), c1 = (int)min((long)c0 + p.chunk, (long)V);
   uint32_t *s_count = s_table, *s_bias = s_table + (r.history ? p.table : 0);
-  int h0 = 0, h1 = 0, b0 = 0, b1 = 0;
+  int h0 = 0, h1 = 0, b0 = 0, b1 = 0, first_h = 0, first_b = 0;
   float rep = 1.0f, pres = 0.0f, freq = 0.0f;
   // the best value, its token, and the first allowed number should all be -infinity (tokens are looked up late)
   float best = -INFINITY;
@@ -113,14 +113,15 @@ __global__ void __launch_bounds__(kPickThreads, 2) logits_pick_kernel(const Pick
       if (r.frequency) freq = r.frequency[m];
       pick_fit(r.n_history, h0, h1, r.bad_flag);
       pick_fit(r.n_bias, b0, b1, r.bad_flag);
+      // the first entries of both lists, most often all of them: one round trip, kept for the later tiles
+      if (h0 + tid < h1) first_h = r.history[h0 + tid];
+      if (b0 + tid < b1) first_b = r.bias_ids[b0 + tid];
     }
     const bool listed = h1 > h0 || b1 > b0;
     if (listed) {
-      // the first entries of both lists, most often all: one round trip
-      const int h = h0 + tid < h1 ? r.history[h0 + tid] : 0, b = b0 + tid < b1 ? r.bias_ids[b0 + tid] : 0;
       auto each = [&](auto &&history, auto &&bias) {
-        for (int i = h0 + tid; i < h1; i += T) history(i == h0 + tid ? h : r.history[i]);
-        for (int i = b0 + tid; i < b1; i += T) bias(i == b0 + tid ? b : r.bias_ids[i], i - b0 + 1);
+        for (int i = h0 + tid; i < h1; i += T) history(i == h0 + tid ? first_h : r.history[i]);
+        for (int i = b0 + tid; i < b1; i += T) bias(i == b0 + tid ? first_b : r.bias_ids[i], i - b0 + 1);
       };
       if (t0 > c0) {
         __syncthreads();  // the previous tile's bits are read

@@ -562,6 +562,9 @@ def run_pick(x, hist=None, rep=None, pres=None, freq=None, bias=None, allow=None
     (1, 151936, 120, 0, False), (3, 151936, 700, 30, True), (5, 1000, 50, 7, True), (2, 1, 3, 1, True),
     (4, 33, 10, 3, True), (9, 4099, 2000, 64, False), (65, 2048, 0, 0, True), (1, 70001, 1, 5, True),
     (2, 31, 0, 4, False),
+    (70, 40000, 900, 9, True), (70, 40001, 600, 9, True),   # two CTAs a row, two tiles each
+    (260, 21000, 40, 3, False),                              # one CTA a row, three tiles
+    (2, 400000, 3000, 40, True), (1, 350001, 30, 0, False),  # more than 16 tiles: several per CTA
 ])
 def test_pick(M, V, n_hist, n_bias, masked):
     rng = np.random.default_rng(M * V)
