@@ -77,8 +77,8 @@ kv_append_int8_kernel(const qasr_kv_int8 c, int layer, const qasr_kv_rows r, con
   constexpr int LPH = HD / 4, HPP = 128 / HD;  // lanes per head, heads per piece
   const int lane = threadIdx.x & 31;
   const unsigned item = blockIdx.x * 8 + (threadIdx.x >> 5), groups = (unsigned)(pieces + per - 1) / per;
+  pdl_wait();  // first: what starts as a dependent of this kernel finds all kernels before it done
   pdl_launch_dependents();
-  pdl_wait();
   if (item == 0) kv_flag_bad(r, c, lane);
   const unsigned row = item / groups;
   if (row >= (unsigned)r.n_rows) return;
@@ -152,8 +152,8 @@ kv_read_int8_kernel(float *__restrict__ k_out, float *__restrict__ v_out, const 
                     const qasr_kv_rows r, int pieces, int per) {
   const int lane = threadIdx.x & 31;
   const unsigned item = blockIdx.x * 8 + (threadIdx.x >> 5), groups = (unsigned)(pieces + per - 1) / per;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   if (item == 0) kv_flag_bad(r, c, lane);
   const unsigned row = item / groups;
   if (row >= (unsigned)r.n_rows) return;

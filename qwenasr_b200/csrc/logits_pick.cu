@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) logits_pick_kernel(const Pick
   for (int i = tid; i < kPickTile / 32; i += T) s_bits[i] = 0;
   __syncthreads();
   cluster_arrive_all();  // waited for before a key is sent: rank 0's barrier is ready
+  pdl_wait();  // first: what starts as a dependent of this kernel finds all kernels before it done
   pdl_launch_dependents();
-  pdl_wait();
   const int rank = (int)cluster_ctarank(), m = blockIdx.y, V = p.vocab;
   const qasr_pick_rules &r = p.r;
   const float *x = p.in + (size_t)m * V;

@@ -135,7 +135,6 @@ struct TaShape {
   static constexpr int kStages = NR == 4 ? 3 : 2;  // K and V tiles in flight
   static constexpr int kGroups = NR == 32 ? 2 : 1;  // softmax warpgroups: each owns R rows of every tile
   static constexpr int kR = NR / kGroups;
-  static constexpr int kChunk = kGroups > 1 ? 8 : kR;  // rows per TMEM load: eight spill less at 96 registers
   static constexpr int kWarps = 4 * kGroups, kThreads = 32 * kWarps + 64;  // and the MMA and the TMA warp
   static constexpr int kQBytes = kN * 128, kPBytes = kN * 128;
 };
@@ -253,7 +252,7 @@ template <int HD, int NR>
 __global__ void __launch_bounds__(TaShape<NR>::kThreads, 2)
 tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
   using Sh = TaShape<NR>;
-  constexpr int HPB = 128 / HD, N = Sh::kN, ST = Sh::kStages, R = Sh::kR, CH = Sh::kChunk;
+  constexpr int HPB = 128 / HD, N = Sh::kN, ST = Sh::kStages, R = Sh::kR;
   constexpr int kMmaWarp = Sh::kWarps, kTmaWarp = Sh::kWarps + 1;
   extern __shared__ unsigned char smem_raw[];
   TaSmem<NR> &sm = *reinterpret_cast<TaSmem<NR> *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -282,8 +281,8 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem, tmem_o = tmem + N;
+  pdl_wait();  // first: what starts as a dependent of this kernel finds all kernels before it done
   pdl_launch_dependents();
-  pdl_wait();
 
   const KvSeq s = kv_seq(p.r, p.c, m);
   const int v0 = (int)(gridDim.y - 1 - blockIdx.y) * NR, rows = min(NR, s.n * W - v0);  // the block's rows v0 .. of s.n * W
@@ -428,18 +427,15 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
     };
     // acc = acc * old + O * coef for the tile whose constants are in rowc[b]
     auto fold = [&](int b) {
+      uint32_t d[3][R];
+      tmem_ld_planes(my_o, NR, d);
 #pragma unroll
-      for (int c0 = 0; c0 < R; c0 += CH) {
-        uint32_t d[3][CH];
-        tmem_ld_planes(my_o + c0, NR, d);
-#pragma unroll
-        for (int i = 0; i < CH; i += 2) {
-          const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(&sm.rowc[b][warp][(c0 + i) / 2][2]);
-          const F2 o = f2_fma(f2((float)(int)d[2][i], (float)(int)d[2][i + 1]), f2(65536.0f, 65536.0f),
-                              f2((float)((int)d[1][i] * 256 + (int)d[0][i]),
-                                 (float)((int)d[1][i + 1] * 256 + (int)d[0][i + 1])));
-          acc2[(c0 + i) / 2] = f2_fma(acc2[(c0 + i) / 2], c.x, f2_mul(o, c.y));
-        }
+      for (int r = 0; r < R; r += 2) {
+        const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(&sm.rowc[b][warp][r / 2][2]);
+        const F2 o =
+            f2_fma(f2((float)(int)d[2][r], (float)(int)d[2][r + 1]), f2(65536.0f, 65536.0f),
+                   f2((float)((int)d[1][r] * 256 + (int)d[0][r]), (float)((int)d[1][r + 1] * 256 + (int)d[0][r + 1])));
+        acc2[r / 2] = f2_fma(acc2[r / 2], c.x, f2_mul(o, c.y));
       }
     };
     // After a timeout (sm.abort) every wait returns at once and the loop runs on: a group's warps must meet at
@@ -455,18 +451,16 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       __syncwarp();
       tc_fence_after();
       float x[R];  // scores in units of log 2
+      {
+        uint32_t d[3][R];
+        tmem_ld_planes(my_s, NR, d);
 #pragma unroll
-      for (int c0 = 0; c0 < R; c0 += CH) {
-        uint32_t d[3][CH];
-        tmem_ld_planes(my_s + c0, NR, d);
-#pragma unroll
-        for (int e = 0; e < CH; e += 2) {
-          const int r = c0 + e;
+        for (int r = 0; r < R; r += 2) {
           const F2 k = f2(HPB == 2 && (my_hi >> r & 1) ? ks[HPB - 1] : ks[0],
                           HPB == 2 && (my_hi >> (r + 1) & 1) ? ks[HPB - 1] : ks[0]);
-          const F2 sum = f2_fma(f2((float)(int)d[0][e], (float)(int)d[0][e + 1]), f2(65536.0f, 65536.0f),
-                                f2((float)((int)d[1][e] * 256 + (int)d[2][e]),
-                                   (float)((int)d[1][e + 1] * 256 + (int)d[2][e + 1])));
+          const F2 sum =
+              f2_fma(f2((float)(int)d[0][r], (float)(int)d[0][r + 1]), f2(65536.0f, 65536.0f),
+                     f2((float)((int)d[1][r] * 256 + (int)d[2][r]), (float)((int)d[1][r + 1] * 256 + (int)d[2][r + 1])));
           const F2 x2 = f2_mul(sum, f2_mul(*reinterpret_cast<const F2 *>(qf + r), k));
           x[r] = f2_lo(x2);
           x[r + 1] = f2_hi(x2);
