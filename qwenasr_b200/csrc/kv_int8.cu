@@ -69,14 +69,15 @@ QASR_DEV uint32_t codes4(float4 x, float inv) {
 
 // Columns of a cache row go in pieces of 128 (one or two heads).  A warp takes
 // `per` pieces of one row, K and V; kPieces of each are in flight together.
+constexpr int kKvThreads = 128, kKvWarps = kKvThreads / 32;  // 32,640 rows: 58 us, 60 with 256 threads, 68 with 512
 template <int HD, int kPieces>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kKvThreads)
 kv_append_int8_kernel(const qasr_kv_int8 c, int layer, const qasr_kv_rows r, const float *__restrict__ k_new,
                       const float *__restrict__ v_new, const int32_t *__restrict__ src_rows, int n_src, int pieces,
                       int per) {
   constexpr int LPH = HD / 4, HPP = 128 / HD;  // lanes per head, heads per piece
   const int lane = threadIdx.x & 31;
-  const unsigned item = blockIdx.x * 8 + (threadIdx.x >> 5), groups = (unsigned)(pieces + per - 1) / per;
+  const unsigned item = blockIdx.x * kKvWarps + (threadIdx.x >> 5), groups = (unsigned)(pieces + per - 1) / per;
   pdl_wait();  // first: what starts as a dependent of this kernel finds all kernels before it done
   pdl_launch_dependents();
   if (item == 0) kv_flag_bad(r, c, lane);
@@ -147,11 +148,11 @@ QASR_DEV float4 dequantize4(uint32_t w, float s) {
 
 // As the append: one warp per `per` pieces of a row.
 template <int HD, int kPieces>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kKvThreads)
 kv_read_int8_kernel(float *__restrict__ k_out, float *__restrict__ v_out, const qasr_kv_int8 c, int layer,
                     const qasr_kv_rows r, int pieces, int per) {
   const int lane = threadIdx.x & 31;
-  const unsigned item = blockIdx.x * 8 + (threadIdx.x >> 5), groups = (unsigned)(pieces + per - 1) / per;
+  const unsigned item = blockIdx.x * kKvWarps + (threadIdx.x >> 5), groups = (unsigned)(pieces + per - 1) / per;
   pdl_wait();
   pdl_launch_dependents();
   if (item == 0) kv_flag_bad(r, c, lane);
@@ -194,8 +195,8 @@ constexpr int kDeep = 4;
 // Small calls are bound by latency: one piece a warp (64 pieces, append and
 // read-back 3.9 us against 5.1 with four; 4408 pieces read in 3.1 against 3.5).
 // From 8192 pieces on four, which quarters the look-ups and keeps 2 to 4 KB per
-// warp in flight (25,856 pieces 17.3 against 22.0 us; 261,120 read in 60.2
-// against 79.7, 5.6 TB/s).
+// warp in flight (25,856 pieces, both calls, 17.3 against 22.0 us; 261,120 read
+// in 58 against 80 us, 5.8 TB/s; two or eight a warp 62 and 66 us).
 struct KvLaunch {
   int pieces, per;
   unsigned grid;
@@ -204,7 +205,7 @@ struct KvLaunch {
     pieces = ceil_div(c.n_kv_heads, 128 / c.head_dim);
     deep = (long)r.n_rows * pieces >= 8192;
     per = deep ? kDeep : 1;
-    grid = (unsigned)ceil_div((long)r.n_rows * ceil_div(pieces, per), 8);
+    grid = (unsigned)ceil_div((long)r.n_rows * ceil_div(pieces, per), kKvWarps);
   }
 };
 
@@ -221,7 +222,7 @@ extern "C" int qasr_kv_append_int8(const qasr_kv_int8 *cache, int layer, const q
   const auto kernel = cache->head_dim == 128
                           ? (l.deep ? kv_append_int8_kernel<128, kDeep> : kv_append_int8_kernel<128, 1>)
                           : (l.deep ? kv_append_int8_kernel<64, kDeep> : kv_append_int8_kernel<64, 1>);
-  const cudaError_t e = launch_pdl(kernel, l.grid, 256, 0, S(stream), *cache, layer, *rows, k_new, v_new, src_rows, n_src,
+  const cudaError_t e = launch_pdl(kernel, l.grid, kKvThreads, 0, S(stream), *cache, layer, *rows, k_new, v_new, src_rows, n_src,
                                    l.pieces, l.per);
   return cuda_status(e, "qasr_kv_append_int8");
 }
@@ -238,6 +239,6 @@ extern "C" int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 
   const auto kernel = cache->head_dim == 128 ? (l.deep ? kv_read_int8_kernel<128, kDeep> : kv_read_int8_kernel<128, 1>)
                                              : (l.deep ? kv_read_int8_kernel<64, kDeep> : kv_read_int8_kernel<64, 1>);
   const cudaError_t e =
-      launch_pdl(kernel, l.grid, 256, 0, S(stream), k_out, v_out, *cache, layer, *rows, l.pieces, l.per);
+      launch_pdl(kernel, l.grid, kKvThreads, 0, S(stream), k_out, v_out, *cache, layer, *rows, l.pieces, l.per);
   return cuda_status(e, "qasr_kv_read_int8");
 }
