@@ -2,7 +2,7 @@
  * qwenasr_cuda.h -- C ABI of the B200 (sm_100a) kernel library for the
  * QwenASR per-layer hot path.
  *
- * Two layers of entry points:
+ * Layers of entry points:
  *
  *  1. Kernel level.  One function per function of the reference's kernel
  *     module (crates/qwen-asr/src/kernels/mod.rs), same argument order and
@@ -13,6 +13,10 @@
  *     QASR_ERR_*), with a message in qasr_last_error().  Fused entries
  *     (qasr_pre_attn_block, qasr_ln_pe, ...) replace a sequence of reference
  *     calls and name the sequence.
+ *
+ *     The serving operators (qasr_kv_append_int8 ... qasr_logits_pick) have no
+ *     counterpart there: an INT8 KV cache, attention of one or several tokens
+ *     per sequence over it, and token picks under rules.
  *
  *  2. Decoder engine.  An opaque qasr_decoder owning INT8 decoder weights on
  *     one GPU, KV caches for a batch of independent sequences and the
@@ -285,7 +289,7 @@ typedef struct {
  * when equal), which stand at rows positions[m] .. of cache slot slots[m]
  * (slots NULL: slot m).  row_starts [n_seqs + 1], positions and slots are
  * device arrays, read when the kernel runs, so a captured call follows their
- * contents.  n_rows: rows of the packed buffers; those from
+ * contents (they must not change while a call runs).  n_rows: rows of the packed buffers; those from
  * row_starts[n_seqs] on are left as they are.  max_rows: at least the rows of
  * the longest sequence (it sizes the launch).  max_keys: how many cache rows
  * the longest sequence may have, if the host knows (0: max_seq); attention
@@ -325,10 +329,13 @@ int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 *cache, int
  * [n_rows]; sequences of at most 64 rows).  tree_mask NULL: j <= t, the
  * causal rule of qasr_causal_attention; with one row per sequence this is a
  * decode step, with many a prompt chunk.  out [n_rows, n_heads * head_dim] =
- * softmax(scale * q k^T) v in f32; a row that sees nothing is zero.  n_heads
- * a multiple of n_kv_heads, at most 64 query heads per kv head; q and out
- * 16-byte aligned.  If a bounded device-side wait gives up, *bad_flag becomes
- * -QASR_ERR_TIMEOUT. */
+ * softmax(scale * q k^T) v in f32; a row that sees nothing is zero, one that
+ * sees a scale of NaN or infinity (or a value scale below 0 or from 2^125 on) is
+ * NaN, and so is the row of a query holding either.  n_heads a multiple of
+ * n_kv_heads, at most 64 query heads per kv head; q and out 16-byte aligned
+ * and without overlap.  No workspace: calls may run at once on any streams.
+ * If a bounded device-side wait gives up, *bad_flag becomes -QASR_ERR_TIMEOUT
+ * and the rows concerned are NaN. */
 int qasr_tree_attention_int8(float *out, const float *q, const qasr_kv_int8 *cache, int layer,
                              const qasr_kv_rows *rows, const uint64_t *tree_mask, int n_heads, float scale,
                              void *stream);
@@ -351,7 +358,7 @@ typedef struct {
 /* Token picks under rules, the step after qasr_final_norm_lmhead_argmax's
  * logits_out.  For every row of logits [M, vocab], per token with value l
  * that appears c times in the row's history:
- *   c > 0:  l > 0 ? l / repetition : l * repetition,
+ *   c > 0:  l > 0 ? l / repetition : l * repetition  (repetition > 0),
  *           minus (presence + frequency * c);
  *   then plus its bias; a token that allow_mask does not allow becomes -inf.
  * logits_out [M, vocab] (NULL, or logits itself, or disjoint from it) receives

@@ -666,6 +666,9 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
   }
 }
 
+// Query rows of one kv head (or pair) of the longest sequence.
+static long longest_rows(const TreeAttnParams &p) { return (long)std::min(p.r.max_rows, p.r.n_rows) * p.width; }
+
 template <int HD, int NR>
 static int tree_attention_launch(TreeAttnParams p, cudaStream_t st) {
   constexpr int HPB = 128 / HD;
@@ -686,11 +689,7 @@ static int tree_attention_launch(TreeAttnParams p, cudaStream_t st) {
     attr_done[dev] = true;
   }
   const int heads = ceil_div(p.c.n_kv_heads, HPB);
-  const long row_blocks = ceil_div((long)p.r.max_rows * p.width, NR);
-  if (row_blocks > 65535) {
-    set_error("qasr_tree_attention_int8: too many query rows per sequence (%d)", p.r.max_rows);
-    return QASR_ERR_UNSUPPORTED;
-  }
+  const long row_blocks = (longest_rows(p) + NR - 1) / NR;  // at most 65,535
   // CTAs per block of rows.  A CTA costs 3 to 4 us beside its tiles, so no more than 256 of them in all (32
   // blocks over 1000 rows: 5.8 us with 8 each, 14.5 with 16; 64 blocks 6.6 with 4, 11.1 with 8), but up to 512
   // where long histories (32 tiles) may differ in length and the longest would set the time: 256 blocks over 250 ..
@@ -721,7 +720,7 @@ static int tree_attention_launch(TreeAttnParams p, cudaStream_t st) {
 
 template <int HD>
 static int tree_attention_rows(const TreeAttnParams &p, cudaStream_t st) {
-  const long rows = (long)p.r.max_rows * p.width;
+  const long rows = longest_rows(p);
   if (rows <= 4) return tree_attention_launch<HD, 4>(p, st);
   if (rows <= 8) return tree_attention_launch<HD, 8>(p, st);
   if (rows <= 16) return tree_attention_launch<HD, 16>(p, st);
@@ -731,15 +730,25 @@ static int tree_attention_rows(const TreeAttnParams &p, cudaStream_t st) {
 // Codes as a [cache rows, kv_dim] byte matrix.
 static int kv_codes_map(CUtensorMap *tm, const int8_t *codes, const qasr_kv_int8 &c) {
   const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
-  if (!encode) return QASR_ERR_CUDA;
+  if (!encode) {
+    set_error("qasr_tree_attention_int8: cuTensorMapEncodeTiled unavailable");
+    return QASR_ERR_CUDA;
+  }
   const cuuint64_t kv_dim = (cuuint64_t)c.n_kv_heads * c.head_dim;
   const cuuint64_t dims[2] = {kv_dim, (cuuint64_t)c.n_slots * c.n_layers * c.max_seq};
   const cuuint64_t strides[1] = {kv_dim};
   const cuuint32_t box[2] = {128, kTaKeys};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(codes), dims, strides, box, estr,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto run = [&] {
+    return encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(codes), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = run();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // this host thread has made no runtime call that binds the device's context
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = run();
+  }
   if (r != CUDA_SUCCESS) {
     set_error("qasr_tree_attention_int8: cuTensorMapEncodeTiled failed (%d)", (int)r);
     return QASR_ERR_CUDA;
@@ -780,17 +789,21 @@ extern "C" int qasr_tree_attention_int8(float *out, const float *q, const qasr_k
   }
   if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return QASR_OK;
   TreeAttnParams p{};
+  p.r = *rows;
+  p.group = n_heads / cache->n_kv_heads;
+  p.width = p.group * (128 / cache->head_dim);
+  if (longest_rows(p) > 32l * 65535) {
+    set_error("qasr_tree_attention_int8: too many query rows per sequence (max_rows %d)", rows->max_rows);
+    return QASR_ERR_UNSUPPORTED;
+  }
   if (int rc = kv_codes_map(&p.tm_k, cache->k, *cache)) return rc;
   if (int rc = kv_codes_map(&p.tm_v, cache->v, *cache)) return rc;
   p.out = out;
   p.q = q;
   p.c = *cache;
-  p.r = *rows;
   p.tree_mask = tree_mask;
   p.layer = layer;
   p.n_heads = n_heads;
-  p.group = n_heads / cache->n_kv_heads;
-  p.width = p.group * (128 / cache->head_dim);
   p.scale = scale;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return cache->head_dim == 128 ? tree_attention_rows<128>(p, st) : tree_attention_rows<64>(p, st);

@@ -268,7 +268,8 @@ def attend_exact(c, layer, q, counts, positions, slots, masks, n_heads, scale):
     return out, bar
 
 
-def check_attend(rng, counts, positions, n_kv, group, hd, tree, size=1.0, pad=1, layers=2, masks=None, max_seq=None):
+def check_attend(rng, counts, positions, n_kv, group, hd, tree, size=1.0, pad=1, layers=2, masks=None, max_seq=None,
+                 max_keys=0):
     n, total, n_heads = len(counts), sum(counts), n_kv * group
     max_seq = max_seq or max(p + r for p, r in zip(positions, counts)) + 3
     c = Cache(rng, n + 1, layers, max_seq, n_kv, hd)
@@ -281,7 +282,7 @@ def check_attend(rng, counts, positions, n_kv, group, hd, tree, size=1.0, pad=1,
     scale = 1.0 / math.sqrt(hd)
     flag = ints([0])
     rows = KvRows(ints(starts_of(counts)), ints(positions), ints(slots), n_rows=total + pad, max_rows=max(counts),
-                  bad_flag=flag)
+                  max_keys=max_keys, bad_flag=flag)
     out = torch.full((total + pad, n_heads * hd), 5.0, device=DEV)
     dev_masks = as_int64(masks + [(1 << 64) - 1] * pad) if tree else None
     K.tree_attention_int8(out, T(q), c.up(), layers - 1, rows, n_heads, scale, dev_masks)
@@ -327,6 +328,14 @@ def test_trees(counts, positions, n_kv, group, hd):
 ])
 def test_chunks(counts, positions, n_kv, group, hd):
     check_attend(np.random.default_rng(sum(positions) + hd), counts, positions, n_kv, group, hd, tree=False)
+
+
+@pytest.mark.parametrize("max_keys", [1, 300, 2100, 1 << 30])
+def test_max_keys_is_a_hint(max_keys):
+    """A bound that is far off changes how the work is split, not what comes out."""
+    rng = np.random.default_rng(max_keys % 1000)
+    check_attend(rng, [1, 1, 1], [2000, 0, 777], 2, 2, 128, tree=False, max_keys=max_keys, max_seq=4100)
+    check_attend(rng, [31], [1900], 1, 2, 64, tree=True, max_keys=max_keys)
 
 
 def test_full_cache():
@@ -484,6 +493,86 @@ def test_graphs_follow_positions():
             K.tree_attention_int8(out, q, dev, 0, rows, n_heads, 0.1)
             torch.cuda.synchronize()
             assert torch.equal(out, replayed[i])
+
+
+def test_first_calls_under_capture():
+    """A process whose very first calls of every operator are captured into a graph."""
+    code = '''
+import torch
+from qwenasr_b200 import kernels as K
+from qwenasr_b200.kvcache import KvCacheInt8, KvRows
+i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+cache = KvCacheInt8.zeros(1, 1, 300, 2, 128)
+rows = KvRows(i32([0, 3]), i32([0]), n_rows=3, max_rows=3)
+k, v, q = torch.randn(3, 256, device="cuda"), torch.randn(3, 256, device="cuda"), torch.randn(3, 512, device="cuda")
+out, back, ids, logits = torch.empty_like(q), torch.empty_like(k), i32([7, 7, 7]), torch.randn(3, 1000, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    K.kv_append_int8(cache, 0, rows, k, v)
+    K.kv_read_int8(back, None, cache, 0, rows)
+    K.tree_attention_int8(out, q, cache, 0, rows, 4, 0.1)
+    K.logits_pick(ids, None, logits, 3, 1000)
+g.replay()
+torch.cuda.synchronize()
+assert ids.tolist() == logits.argmax(1).tolist()
+assert (back - k).abs().max() <= k.abs().max() / 127 and torch.isfinite(out).all()
+g2, o2 = out.clone(), out.zero_()
+K.tree_attention_int8(out, q, cache, 0, rows, 4, 0.1)
+assert torch.equal(out, g2)
+print("captured")
+'''
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_host_threads():
+    """Calls from two threads on two streams at once, over one cache: each gets what it gets alone."""
+    import threading
+    rng = np.random.default_rng(14)
+    c = Cache(rng, 2, 1, 600, 2, 128)
+    for sl in range(2):
+        c.fill(rng, sl, 0, 600)
+    dev = c.up()
+    work = []
+    for sl in range(2):
+        q = T(rng.standard_normal((40, 512)).astype(np.float32))
+        rows = KvRows(ints([0, 40]), ints([500 + sl]), ints([sl]), n_rows=40, max_rows=40)
+        logits = T(rng.standard_normal((3, 5000)).astype(np.float32))
+        work.append((q, rows, torch.empty_like(q), logits, ints([0, 0, 0]), torch.cuda.Stream()))
+    alone = []
+    for q, rows, out, logits, ids, _ in work:
+        K.tree_attention_int8(out, q, dev, 0, rows, 4, 0.1)
+        K.logits_pick(ids, None, logits, 3, 5000)
+        alone.append((out.clone(), ids.clone()))
+        out.zero_()
+        ids.zero_()
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        q, rows, out, logits, ids, s = work[i]
+        try:
+            with torch.cuda.stream(s):
+                for _ in range(50):
+                    K.tree_attention_int8(out, q, dev, 0, rows, 4, 0.1)
+                    K.logits_pick(ids, None, logits, 3, 5000)
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for (q, rows, out, logits, ids, s), (o, n) in zip(work, alone):
+        assert torch.equal(out, o) and torch.equal(ids, n)
 
 
 def test_wrong_device_and_shapes_raise():

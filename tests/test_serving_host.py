@@ -105,6 +105,8 @@ def test_attention_refusals(lib):
     assert attend(r=rows(max_rows=65), mask=P) == _lib.QASR_ERR_UNSUPPORTED
     assert "64 rows" in _lib.last_error()
     assert attend(r=rows(n_seqs=70000)) == _lib.QASR_ERR_UNSUPPORTED
+    assert attend(r=rows(max_rows=1 << 30, n_rows=1 << 27)) == _lib.QASR_ERR_UNSUPPORTED
+    assert "query rows" in _lib.last_error()
 
 
 def test_pick_refusals(lib):
