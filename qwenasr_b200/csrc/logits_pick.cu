@@ -168,18 +168,17 @@ __global__ void __launch_bounds__(kPickThreads, 2) logits_pick_kernel(const Pick
         else
 #pragma unroll
           for (int e = 0; e < 4; ++e) hit |= (s_bits[place(k, e) >> 5] >> (place(k, e) & 31) & 1) << e;
-        if (hit) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (!(hit >> e & 1)) continue;
-            float l = v[k][e];
-            if (const uint32_t c = r.history ? s_count[place(k, e)] : 0) {
-              l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
-              l = __fsub_rn(l, __fadd_rn(pres, __fmul_rn(freq, (float)c)));
-            }
-            if (const uint32_t c = r.bias_ids ? s_bias[place(k, e)] : 0) l = __fadd_rn(l, r.bias_values[b0 + c - 1]);
-            v[k][e] = l;
+        while (hit) {  // one at a time: seldom more in a warp's 128 tokens
+          const int e = __ffs(hit) - 1, i = place(k, 0) + (VEC ? e : e * T);
+          hit &= hit - 1;
+          float l = e == 0 ? v[k][0] : e == 1 ? v[k][1] : e == 2 ? v[k][2] : v[k][3];
+          if (const uint32_t c = r.history ? s_count[i] : 0) {
+            l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
+            l = __fsub_rn(l, __fadd_rn(pres, __fmul_rn(freq, (float)c)));
           }
+          if (const uint32_t c = r.bias_ids ? s_bias[i] : 0) l = __fadd_rn(l, r.bias_values[b0 + c - 1]);
+#pragma unroll
+          for (int f = 0; f < 4; ++f) v[k][f] = e == f ? l : v[k][f];
         }
       }
       if constexpr (MASK) {

@@ -95,31 +95,6 @@ QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][1
       : "memory");
 }
 
-// Two f32 in one register pair: rows go two at a time through the f32 steps.
-using F2 = unsigned long long;
-QASR_DEV F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-QASR_DEV float f2_lo(F2 a) { return __uint_as_float((uint32_t)a); }
-QASR_DEV float f2_hi(F2 a) { return __uint_as_float((uint32_t)(a >> 32)); }
-QASR_DEV F2 f2_add(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-QASR_DEV F2 f2_mul(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-QASR_DEV F2 f2_fma(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 constexpr int kTaKeys = 128;             // keys of a tile: TMEM lanes of S^T
 constexpr int kTaTile = kTaKeys * 128;   // bytes of a K (or V) tile
 constexpr int kTaMaxCluster = 16;
