@@ -2,6 +2,7 @@
 
     from qwenasr_b200 import kernels      # mirror of crates/qwen-asr/src/kernels
     from qwenasr_b200.decoder import Decoder   # INT8 decoder engine (decode step)
+    from qwenasr_b200.kvcache import KvCacheInt8, KvRows   # INT8 KV cache of the serving operators
 
 The compute lives in libqwenasr_b200.so (C ABI: include/qwenasr_cuda.h),
 built in-tree by `python -m qwenasr_b200.build`.
