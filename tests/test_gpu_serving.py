@@ -654,6 +654,8 @@ def run_pick(x, hist=None, rep=None, pres=None, freq=None, bias=None, allow=None
     (70, 40000, 900, 9, True), (70, 40001, 600, 9, True),   # two CTAs a row, two tiles each
     (260, 21000, 40, 3, False),                              # one CTA a row, three tiles
     (2, 400000, 3000, 40, True), (1, 350001, 30, 0, False),  # more than 16 tiles: several per CTA
+    (257, 20000, 14000, 6, False),                           # most of the vocabulary listed
+    (300, 270000, 5, 3, False),                              # one CTA a row, 27 tiles
 ])
 def test_pick(M, V, n_hist, n_bias, masked):
     rng = np.random.default_rng(M * V)
