@@ -338,6 +338,16 @@ def test_max_keys_is_a_hint(max_keys):
     check_attend(rng, [31], [1900], 1, 2, 64, tree=True, max_keys=max_keys)
 
 
+@pytest.mark.parametrize("counts,group,hd,tree", [
+    ([1, 1], 2, 128, False), ([1], 4, 64, False), ([4], 2, 128, True), ([7], 2, 128, True), ([5], 3, 64, True),
+    ([16], 2, 128, True), ([40], 1, 64, True), ([33], 2, 128, False),
+])
+def test_many_tiles_per_cta(counts, group, hd, tree):
+    """With the hint at one key nothing is split: a dozen tiles and more go through one CTA's ring."""
+    rng = np.random.default_rng(group * hd + sum(counts))
+    check_attend(rng, counts, [1500 + 130 * i for i in range(len(counts))], 2, group, hd, tree=tree, max_keys=1)
+
+
 def test_full_cache():
     check_attend(np.random.default_rng(1), [2, 1], [126, 127], 2, 2, 128, tree=False, max_seq=128, pad=0)
 
