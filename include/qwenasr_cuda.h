@@ -352,7 +352,8 @@ typedef struct {
   const int32_t *bias_starts;
   int n_bias;
   const uint32_t *allow_mask; /* [M, ceil(vocab / 32)]: bit t % 32 of word t / 32 set = token t allowed */
-  int32_t *bad_flag;          /* set to 1 by a list or token out of range (that list or entry is ignored) */
+  int32_t *bad_flag;          /* set to 1 by a list or token out of range (that list or entry is ignored), to
+                                 -QASR_ERR_TIMEOUT if a bounded device-side wait gives up (the row's id is -1) */
 } qasr_pick_rules;
 
 /* Token picks under rules, the step after qasr_final_norm_lmhead_argmax's

@@ -34,9 +34,9 @@ QASR_DEV void pick_fit(int n, int &a, int &b, int32_t *bad) {
 }
 
 // One cluster per row; each CTA takes `chunk` tokens in tiles of kPickTile
-// (one, for 16 CTAs and up to 163,840 tokens).  HBM-bound by design: a thread's logits and mask
-// bits of the tile are requested first, and while they are on their way the
-// row's lists, few against its tokens, are read by every CTA, which keeps what
+// (one, for 16 CTAs and up to 163,840 tokens).  HBM-bound by design: a thread's
+// logits and mask bits of the tile are requested first, and while they are on
+// their way the row's lists, few against its tokens, are read by every CTA, which keeps what
 // falls into its tile: a bit per token that has an entry at all, counts by integer
 // atomics (no order), the bias as the largest list index (the last entry for a
 // token).  The tables are cleared at the listed tokens only.  Tokens with an
@@ -49,7 +49,8 @@ QASR_DEV void pick_fit(int n, int &a, int &b, int32_t *bad) {
 // (loads, instructions and stores of four tiles one after the other; 18 us
 // without mask and bias).
 // VEC: rows start on 16-byte boundaries; a quad is four neighbours, loaded as
-// one.  Otherwise its elements lie kPickThreads apart, each load coalesced.
+// one.  Otherwise its elements lie kPickThreads apart, each load coalesced (no
+// rules, 8 rows 3.9 and 4.5 us, 64 rows 14.6 and 16.4).
 // MASK: the rules have a mask of allowed tokens.
 template <bool VEC, bool MASK>
 __global__ void __launch_bounds__(kPickThreads, 2) logits_pick_kernel(const PickParams p) {

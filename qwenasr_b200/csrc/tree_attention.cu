@@ -676,11 +676,12 @@ static int tree_attention_launch(TreeAttnParams p, cudaStream_t st) {
   }
   const int heads = ceil_div(p.c.n_kv_heads, HPB);
   const long row_blocks = (longest_rows(p) + NR - 1) / NR;  // at most 65,535
-  // CTAs per block of rows.  A CTA costs 3 to 4 us beside its tiles, so no more than 256 of them in all (32
-  // blocks over 1000 rows: 5.8 us with 8 each, 14.5 with 16; 64 blocks 6.6 with 4, 11.1 with 8), but up to 512
-  // where long histories (32 tiles) may differ in length and the longest would set the time: 256 blocks over 250 ..
-  // 8000 rows take 48 us with two each and 61 with one (all 8000: 88 and 82).  Sixteen of a cluster find room on
-  // few SMs of a GPC at a time: only for 8 blocks (2000 rows: 5.4 us, 5.8 with 8; 16 blocks 9.6 and 5.3).
+  // CTAs per block of rows.  A CTA costs 3 to 4 us beside its tiles, so no more than 256 of them in all (over 1000
+  // rows, 32 blocks take 5.9 us with 8 each and 14.1 with 16; 64 blocks 6.5 with 4, 11.3 with 8), but up to 512 where
+  // long histories (32 tiles) may differ in length and the longest would set the time: 256 blocks over 250 .. 8000 rows
+  // take 47 us with two each and 62 with one (all 8000: 87 and 81); 128 blocks 30 with four and 36 with two (50 and
+  // 44).  Sixteen of a cluster find room on few SMs of a GPC at a time: only for 8 blocks (2000 rows: 5.6 us, 5.7 with
+  // 8; 16 blocks 9.4 and 5.5).
   const int keys = p.r.max_keys > 0 ? std::min(p.r.max_keys, p.c.max_seq) : p.c.max_seq;
   const int tiles = ceil_div(keys, kTaKeys);
   const long blocks = (long)heads * row_blocks * p.r.n_seqs;
