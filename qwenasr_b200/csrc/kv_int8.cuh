@@ -80,6 +80,11 @@ QASR_DEV F2 f2_add(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+QASR_DEV F2 f2_add_up(F2 a, F2 b) {  // rounded up
+  F2 r;
+  asm("add.rp.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 QASR_DEV F2 f2_mul(F2 a, F2 b) {
   F2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));

@@ -13,13 +13,17 @@
 //    digits, as in the INT8 projections.  S^T [keys x 3 digit planes of the
 //    rows] = K codes [128 keys x 128] * digits^T; the rounding of q is half a
 //    step of 2^-22 of the row's largest magnitude.
-//  * a weight e^(S - tile maximum) * vs_j / (the tile's largest vs) lies in
-//    [0, 1]; 2^23 times it, rounded, are three unsigned digits (the low bytes of
-//    the float 2^23 + that), off by at most 2^-24 of the largest weight and
-//    value scale of the tile, below the f32 rounding of a sum over it.  O^T [128
-//    values x digit planes] = V codes^T * digits, with V read as it lies
-//    (M-major) and the digits written by the thread that owns the key (N-major):
-//    nothing is transposed or converted on the way.
+//  * a product e^S_tj * vs_j over the largest one that the row sees in the tile
+//    lies in [0, 1]; 2^22.998 times it, rounded, are three unsigned digits (the
+//    low bytes of the float 2^23 + that), off by at most 2^-23.9 of the largest
+//    product.  Many products of the tile's largest size add up to an error of
+//    some 2^-22 of their sum, about that of f32 sums.  The reference is the row's
+//    own and the product's: with the largest weight and the largest scale, each
+//    for itself, a sink (much weight, small values) or the scale of a key that
+//    the row does not see would take the bits of all others.  O^T [128 values x
+//    digit planes] = V codes^T * digits, with V read as it lies (M-major) and the
+//    digits written by the thread that owns the key (N-major): nothing is
+//    transposed or converted on the way.
 // Digit sums are recombined in f32 (one rounding below the value's own) and
 // accumulated over the tiles in f32 with the usual running maximum and sum.
 //
@@ -147,10 +151,11 @@ struct TaSmem {
   // partial states pushed by the cluster: entry r / C * C + c is CTA c's of row r, one of the rows r % C = rank
   static constexpr int kRecv = NR < kTaMaxCluster ? kTaMaxCluster : NR;
   float recv[kRecv][128], recv_m[kRecv], recv_l[kRecv];
-  // per tile (two in flight), warp and pair of rows: minus the tile maximum, the factors of the tile's sum, of the
-  // sums before it and of O
+  // per tile (two in flight), warp and pair of rows: minus the running maximum, units per weight, the factor of the
+  // sums before the tile, what a unit of O counts
   alignas(16) F2 rowc[2][Sh::kWarps][Sh::kR / 2][4];
-  alignas(16) float wmax[2][Sh::kWarps][Sh::kR + 4];  // per tile and warp: row maxima, then the largest value scales
+  // per tile and warp: the rows' largest scores, then their largest products of weight and value scale (log 2)
+  alignas(16) float wmax[2][Sh::kWarps][2 * Sh::kR];
   alignas(16) float qf[NR];  // 2^(E-22) * scale * log2(e)
   float lsum[4][NR], mrun[NR];
   uint32_t mask[2][NR];
@@ -179,6 +184,11 @@ constexpr uint32_t ta_idesc_o(int N) {
 QASR_DEV float ta_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+QASR_DEV float ta_lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 QASR_DEV float ta_rcp(float x) {
@@ -470,21 +480,30 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       }
       // a value scale that is no number in [0, 2^125) counts as NaN, for the rows that see it
       bool odd[HPB];
-      float top[R + 4];  // the warp's row maxima, then those of the value scales
-#pragma unroll
-      for (int r = 0; r < R; ++r) top[r] = ta_warp_max(x[r]);
+      float lvs[HPB];
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
         odd[u] = !(vs[u] >= 0.0f && vs[u] < 4.2535296e37f);
         if (odd[u]) vs[u] = 0.0f;
-        top[R + u] = ta_warp_max(vs[u]);
+        lvs[u] = ta_lg2(vs[u]);
       }
+      // Of two heads' values the one of row r.  The bits pass through a register that the compiler knows nothing of,
+      // or it keeps the choice of all rows at hand and spills 80 bytes for it (32 rows: 28.7 us against 26.4).
+      uint32_t second = my_hi;
+      if constexpr (HPB == 2) asm volatile("" : "+r"(second));
+      auto of_row = [&](const float(&a)[HPB], int r) { return HPB == 2 && (second >> r & 1) ? a[HPB - 1] : a[0]; };
 #pragma unroll
-      for (int u = HPB; u < 4; ++u) top[R + u] = 0.0f;
-      if (lane == 0) {
-#pragma unroll
-        for (int r = 0; r < R + 4; r += 4)
-          *reinterpret_cast<float4 *>(&sm.wmax[buf][warp][r]) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
+      for (int r = 0; r < R; r += 4) {  // the warp's maxima; products' logarithms rounded up: none passes its maximum
+        const F2 a = f2_add_up(f2(x[r], x[r + 1]), f2(of_row(lvs, r), of_row(lvs, r + 1)));
+        const F2 b = f2_add_up(f2(x[r + 2], x[r + 3]), f2(of_row(lvs, r + 2), of_row(lvs, r + 3)));
+        const float4 s4 =
+            make_float4(ta_warp_max(x[r]), ta_warp_max(x[r + 1]), ta_warp_max(x[r + 2]), ta_warp_max(x[r + 3]));
+        const float4 u4 =
+            make_float4(ta_warp_max(f2_lo(a)), ta_warp_max(f2_hi(a)), ta_warp_max(f2_lo(b)), ta_warp_max(f2_hi(b)));
+        if (lane == 0) {
+          *reinterpret_cast<float4 *>(&sm.wmax[buf][warp][r]) = s4;
+          *reinterpret_cast<float4 *>(&sm.wmax[buf][warp][R + r]) = u4;
+        }
       }
       named_bar(2 + wg, 128);
       const int w0 = 4 * wg;  // the group's warps
@@ -492,25 +511,20 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         return fmaxf(fmaxf(sm.wmax[buf][w0][e], sm.wmax[buf][w0 + 1][e]),
                      fmaxf(sm.wmax[buf][w0 + 2][e], sm.wmax[buf][w0 + 3][e]));
       };
-      // Value scales relative to the tile's largest, times 2^23: a weight's integer is e^(S - max) * vs / largest *
-      // 2^23, its last rounding half a unit.  The reciprocal's own error scales the whole tile, by an ulp or two.
-      float step[HPB];  // what a unit counts
-#pragma unroll
-      for (int u = 0; u < HPB; ++u) {
-        const float t = fmaxf(over_warps(R + u), 7.888609e-31f);  // 2^-100: below it values lose bits instead
-        step[u] = __fmul_rn(t, 1.0f / kTaMagic);
-        vs[u] = __fmul_rn(vs[u], __fmul_rn(kTaMagic, ta_rcp(t)));
-      }
+      // A product's integer is 2^(x - base) * vs * units, at most 2^23: 2^22.998 leaves room for the errors of the
+      // logarithms and exponentials (below 2^-13 in all) and for the roundings.  What a unit counts is the reciprocal
+      // of `units`, to an ulp or two that scales the whole tile's share.
+      const float most = lane < 2 * R ? over_warps(lane) : 0.0f, umax = __shfl_down_sync(0xffffffffu, most, R);
       if (lane < R) {
-        const float t = over_warps(lane);
-        const float top = fmaxf(m_run, t), base = top == -INFINITY ? 0.0f : top;
-        const float f = t == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(t, base));
+        const float top = fmaxf(m_run, most), base = top == -INFINITY ? 0.0f : top;
         const float old = m_run == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(m_run, base));
+        // a tile whose products are all below 2^-100 of the row's largest weight loses bits
+        const float units = ta_ex2(__fadd_rn(fminf(__fsub_rn(base, umax), 100.0f), 22.998f));
         float *c = reinterpret_cast<float *>(sm.rowc[buf][warp][lane / 2]) + lane % 2;
-        c[0] = t == -INFINITY ? 0.0f : -t;
-        c[2] = f;
+        c[0] = -base;
+        c[2] = units;
         c[4] = old;
-        c[6] = __fmul_rn(f, HPB == 2 && (my_hi >> lane & 1) ? step[HPB - 1] : step[0]);
+        c[6] = ta_rcp(units);
         m_run = top;
       }
       __syncwarp();
@@ -542,10 +556,8 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
           const F2 old = sm.rowc[buf][warp][r / 2][2];
           const F2 y = f2_add(f2(x[r], x[r + 1]), c.x);
           const F2 pr = f2(ta_ex2(f2_lo(y)), ta_ex2(f2_hi(y)));
-          l2[r / 2] = f2_fma(l2[r / 2], old, f2_mul(pr, c.y));
-          const F2 v = f2(HPB == 2 && (my_hi >> r & 1) ? vs[HPB - 1] : vs[0],
-                          HPB == 2 && (my_hi >> (r + 1) & 1) ? vs[HPB - 1] : vs[0]);
-          const F2 w2 = f2_fma(pr, v, f2(kTaMagic, kTaMagic));
+          l2[r / 2] = f2_fma(l2[r / 2], old, pr);
+          const F2 w2 = f2_fma(f2_mul(pr, f2(of_row(vs, r), of_row(vs, r + 1))), c.y, f2(kTaMagic, kTaMagic));
           f[e] = (uint32_t)w2;
           f[e + 1] = (uint32_t)(w2 >> 32);
         }
