@@ -1,5 +1,5 @@
 """The 2-norm bar of attention over the INT8 cache, on the CPU: a model of the kernel's arithmetic keeps it, and
-a model that scales the weights by keys that a row does not see does not."""
+models that lose a plane of digits, or scale the weights by keys that a row does not see, do not."""
 import numpy as np
 import pytest
 
@@ -24,6 +24,12 @@ def shares(kind, n, hd, hide=0, **kw):
                                   "outlier3"])
 def test_the_arithmetic_keeps_the_bar(kind, n, hd):
     assert (shares(kind, n, hd) < 1).all()
+
+
+@pytest.mark.parametrize("n,hd", SIZES[1:])
+@pytest.mark.parametrize("lose", ["q", "w"])
+def test_a_lost_plane_of_digits_does_not(lose, n, hd):
+    assert (shares("plain", n, hd, lose=lose) > 1).all()
 
 
 @pytest.mark.parametrize("n,hd", [(5, 64), (128, 128), (545, 128), (3001, 128)])  # the hidden key shares a tile
