@@ -441,7 +441,10 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       const int buf = i & 1, j = (i0 + i) * kTaKeys + col;
       float ks[HPB], vs[HPB];
 #pragma unroll
-      for (int u = 0; u < HPB; ++u) ks[u] = nks[u], vs[u] = nvs[u];
+      for (int u = 0; u < HPB; ++u) {
+        ks[u] = fmaf(nks[u], 0.0f, nks[u]);  // an infinity becomes NaN: a score of -infinity would count as hidden
+        vs[u] = nvs[u];
+      }
       load_scales(i + 1 < n);
       ta_wait(sm, &sm.sfull, (unsigned)(i & 1));
       __syncwarp();
