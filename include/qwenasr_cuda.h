@@ -296,7 +296,8 @@ typedef struct {
  * splits its work by it, results do not depend on it.  A sequence whose entries do
  * not fit (rows outside the packed buffers or the cache, more than max_rows
  * rows, a slot outside the cache) is left out, its outputs unwritten, and sets
- * *bad_flag (device, may be NULL; never cleared) to 1. */
+ * *bad_flag (device, may be NULL; never cleared) to 1.  A call without
+ * sequences or rows does nothing, whatever its other pointers. */
 typedef struct {
   const int32_t *row_starts, *positions, *slots;
   int n_seqs, n_rows, max_rows, max_keys;
@@ -346,7 +347,9 @@ int qasr_tree_attention_int8(float *out, const float *q, const qasr_kv_int8 *cac
 
 /* Rules of qasr_logits_pick; every pointer is a device pointer and may be
  * NULL (that rule is off).  Lists are packed: row m owns entries starts[m] ..
- * starts[m+1]-1 (starts [M + 1]) of an array of n_... entries. */
+ * starts[m+1]-1 (starts [M + 1]) of an array of n_... entries.  A list of no
+ * entries is one too, with or without an address, as long as it has starts: a
+ * batch's first picks have penalties and an empty history. */
 typedef struct {
   const int32_t *history, *history_starts; /* tokens so far; a token may appear often */
   int n_history;

@@ -222,12 +222,12 @@ struct KvLaunch {
 extern "C" int qasr_kv_append_int8(const qasr_kv_int8 *cache, int layer, const qasr_kv_rows *rows, const float *k_new,
                                    const float *v_new, const int32_t *src_rows, int n_src, void *stream) {
   if (int rc = kv_int8_check("qasr_kv_append_int8", cache, layer, rows)) return rc;
+  if (rows->n_seqs == 0 || rows->n_rows == 0) return QASR_OK;  // empty operands have no address
   if (!k_new || !v_new || !al16(k_new) || !al16(v_new) || n_src < 0 || (!src_rows && n_src < rows->n_rows)) {
     set_error("qasr_kv_append_int8: k_new and v_new must be 16-byte aligned and hold n_rows = %d rows (n_src = %d) "
               "unless src_rows picks them", rows->n_rows, n_src);
     return QASR_ERR_INVALID;
   }
-  if (rows->n_seqs == 0 || rows->n_rows == 0) return QASR_OK;
   const KvLaunch l(*cache, *rows);
   const auto kernel = cache->head_dim == 128
                           ? (l.deep ? kv_append_int8_kernel<128, kDeep> : kv_append_int8_kernel<128, 1>)
@@ -240,11 +240,11 @@ extern "C" int qasr_kv_append_int8(const qasr_kv_int8 *cache, int layer, const q
 extern "C" int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 *cache, int layer,
                                  const qasr_kv_rows *rows, void *stream) {
   if (int rc = kv_int8_check("qasr_kv_read_int8", cache, layer, rows)) return rc;
+  if (rows->n_seqs == 0 || rows->n_rows == 0) return QASR_OK;
   if ((!k_out && !v_out) || !al16(k_out) || !al16(v_out)) {
     set_error("qasr_kv_read_int8: k_out or v_out must be given, 16-byte aligned");
     return QASR_ERR_INVALID;
   }
-  if (rows->n_seqs == 0 || rows->n_rows == 0) return QASR_OK;
   const KvLaunch l(*cache, *rows);
   const auto kernel = cache->head_dim == 128 ? (l.deep ? kv_read_int8_kernel<128, kDeep> : kv_read_int8_kernel<128, 1>)
                                              : (l.deep ? kv_read_int8_kernel<64, kDeep> : kv_read_int8_kernel<64, 1>);

@@ -270,11 +270,21 @@ using namespace qasr;
 
 extern "C" int qasr_logits_pick(int32_t *ids, float *logits_out, const float *logits, const qasr_pick_rules *rules,
                                 int M, int vocab, void *stream) {
-  if (!logits || (!ids && !logits_out) || !rules || M < 0 || vocab <= 0) {
-    set_error("qasr_logits_pick: invalid arguments (null logits or rules, no output, M=%d, vocab=%d)", M, vocab);
+  if (!rules || M < 0 || vocab <= 0) {
+    set_error("qasr_logits_pick: invalid arguments (null rules, M=%d, vocab=%d)", M, vocab);
     return QASR_ERR_INVALID;
   }
-  const qasr_pick_rules &r = *rules;
+  if (M == 0) return QASR_OK;  // before the pointers are looked at: an empty tensor has none
+  if (!logits || (!ids && !logits_out)) {
+    set_error("qasr_logits_pick: null logits or no output");
+    return QASR_ERR_INVALID;
+  }
+  qasr_pick_rules r = *rules;
+  // An empty list has no address of its own: it goes by any other, of which nothing is read (every row's range of it
+  // is empty or flagged).
+  if (!r.history && r.n_history == 0) r.history = r.history_starts;
+  if (!r.bias_ids && r.n_bias == 0) r.bias_ids = r.bias_starts;
+  if (r.bias_ids && !r.bias_values && r.n_bias == 0) r.bias_values = reinterpret_cast<const float *>(r.bias_starts);
   if ((r.history && (!r.history_starts || r.n_history < 0)) ||
       (r.bias_ids && (!r.bias_values || !r.bias_starts || r.n_bias < 0))) {
     set_error("qasr_logits_pick: history needs history_starts, bias_ids need bias_values and bias_starts");
@@ -288,7 +298,6 @@ extern "C" int qasr_logits_pick(int32_t *ids, float *logits_out, const float *lo
     set_error("qasr_logits_pick: at most 65535 rows and 2^30 tokens (M=%d, vocab=%d)", M, vocab);
     return QASR_ERR_UNSUPPORTED;
   }
-  if (M == 0) return QASR_OK;
   PickParams p{ids, logits_out, logits, r, vocab, 0, 0};
   // CTAs per row: as many as 16, one tile each, while all CTAs run at once (two on an SM; clusters of 16 leave part
   // of a GPC's SMs idle).  Vocabulary 151,936, us with 16 / 8 / 4 CTAs a row: 1 row 4.0 / 5.4 / 8.6, 8 rows 4.9 /

@@ -770,6 +770,7 @@ extern "C" int qasr_tree_attention_int8(float *out, const float *q, const qasr_k
                                         const qasr_kv_rows *rows, const uint64_t *tree_mask, int n_heads, float scale,
                                         void *stream) {
   if (int rc = kv_int8_check("qasr_tree_attention_int8", cache, layer, rows)) return rc;
+  if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return QASR_OK;  // empty operands have no address
   if (!out || !q || out == q || (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(q) & 15) ||
       (reinterpret_cast<uintptr_t>(tree_mask) & 7)) {
     set_error("qasr_tree_attention_int8: q and out must be distinct and 16-byte aligned, tree_mask 8-byte aligned");
@@ -793,7 +794,6 @@ extern "C" int qasr_tree_attention_int8(float *out, const float *q, const qasr_k
     set_error("qasr_tree_attention_int8: at most 65535 sequences (%d)", rows->n_seqs);
     return QASR_ERR_UNSUPPORTED;
   }
-  if (rows->n_seqs == 0 || rows->n_rows == 0 || rows->max_rows == 0) return QASR_OK;
   TreeAttnParams p{};
   p.r = *rows;
   p.group = n_heads / cache->n_kv_heads;

@@ -341,12 +341,15 @@ def logits_pick(ids_out, logits_out, logits, M, vocab, history=None, history_sta
     """Penalties of repeated tokens, biases and the mask of allowed tokens on
     logits [M, vocab], then the first-max pick (qasr_logits_pick).  ids_out or
     logits_out may be None; logits_out may be logits.  Lists are packed with
-    starts [M + 1]; allow_mask is int32 [M, ceil(vocab / 32)], bit set = allowed."""
+    starts [M + 1] and may be empty; allow_mask is int32 [M, ceil(vocab / 32)], bit set = allowed."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
     dev = logits.get_device()
     n_hist = 0 if history is None else history.numel()
     n_bias = 0 if bias_ids is None else bias_ids.numel()
+    if history is None or bias_ids is None:  # without its list a rule is off, whatever its starts
+        history_starts = None if history is None else history_starts
+        bias_starts = None if bias_ids is None else bias_starts
     r = _lib.PickRules(_need(history, i32, dev, "history", 0), _need(history_starts, i32, dev, "history_starts", M + 1),
                        n_hist, _need(repetition, f32, dev, "repetition", M), _need(presence, f32, dev, "presence", M),
                        _need(frequency, f32, dev, "frequency", M), _need(bias_ids, i32, dev, "bias_ids", 0),

@@ -145,3 +145,24 @@ def test_python_faces_refuse_host_tensors():
     from qwenasr_b200 import kernels as K
     with pytest.raises(ValueError, match="CUDA"):
         K.logits_pick(None, None, torch.zeros(1, 8), 1, 8)
+
+
+def test_empty_operands_have_no_address(lib):
+    """What an empty tensor hands over, a null pointer, is no error in an empty call."""
+    for r in (rows(n_seqs=0, row_starts=None, positions=None), rows(n_rows=0)):
+        assert lib.qasr_kv_append_int8(cache(), 1, r, None, None, None, 0, None) == _lib.QASR_OK
+        assert lib.qasr_kv_read_int8(None, None, cache(), 1, r, None) == _lib.QASR_OK
+        assert lib.qasr_tree_attention_int8(None, None, cache(), 1, r, None, 16, 0.1, None) == _lib.QASR_OK
+    rules = _lib.PickRules(history_starts=256, repetition=256, bias_starts=256)
+    assert lib.qasr_logits_pick(None, None, None, C.byref(rules), 0, 100, None) == _lib.QASR_OK
+
+
+def test_penalties_of_an_empty_history_pass_the_checks(lib):
+    """They get as far as the limit of rows, as those of any history do."""
+    def pick(**kw):
+        return lib.qasr_logits_pick(P, None, P, C.byref(_lib.PickRules(**kw)), 70000, 100, None)
+
+    assert pick(history_starts=256, repetition=256, presence=256, frequency=256) == _lib.QASR_ERR_UNSUPPORTED
+    assert pick(bias_starts=256) == _lib.QASR_ERR_UNSUPPORTED
+    assert pick(history_starts=256, n_history=2, repetition=256) == _lib.QASR_ERR_INVALID  # entries without a list
+    assert pick(repetition=256) == _lib.QASR_ERR_INVALID
