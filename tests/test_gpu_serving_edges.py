@@ -1,9 +1,10 @@
-"""The serving operators at their edges: scales that are no numbers, empty batches and lists."""
+"""The serving operators at their edges: scales that are no numbers, empty batches and lists, the variant of long calls."""
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_serving import (Cache, DEV, H, KvCacheInt8, KvRows, T, as_int64, attend_exact, ints, pack, pick_ref)
+from test_gpu_serving import (Cache, DEV, H, KvCacheInt8, KvRows, T, as_int64, attend_exact, ints, pack, pick_ref,
+                              quantize, starts_of)
 
 from qwenasr_b200 import kernels as K
 
@@ -95,3 +96,45 @@ def test_no_history_yet():
     f = np.float32
     ref_ids, ref = pick_ref(x, [[], [5, 6, 5], []], np.full(3, 2, f), np.ones(3, f), np.ones(3, f), None, None)
     assert np.array_equal(H(ids), ref_ids) and np.array_equal(H(out), ref)
+
+
+# ---------------------------------------------------- long calls, bit by bit --
+def pieces(n_kv, hd):
+    return -(-n_kv * hd // 128)
+
+
+@pytest.mark.parametrize("n_kv,hd", [(5, 128), (8, 128), (9, 64), (11, 64), (1, 128), (7, 64)])
+@pytest.mark.parametrize("beyond", [-1, 0, 1, 700])  # rows around the one where calls go four pieces a warp
+@pytest.mark.parametrize("gather", [False, True])
+def test_long_calls(n_kv, hd, beyond, gather):
+    rng = np.random.default_rng(n_kv * hd + beyond + 1)
+    total, pad, d = -(-8192 // pieces(n_kv, hd)) + beyond, 3, n_kv * hd
+    counts = [total // 3, 0, total - total // 3 - 5, 5]
+    max_seq, layer = max(counts) + 9, 1
+    cache = KvCacheInt8.zeros(4, 2, max_seq, n_kv, hd)
+    n_src = total + (50 if gather else pad)
+    k, v = ((rng.standard_normal((n_src, d)) * np.exp(rng.normal(0, 2, (n_src, 1)))).astype(np.float32) for _ in range(2))
+    src = rng.permutation(n_src)[:total] if gather else np.arange(total)
+    k[src[7], :hd] = np.nan                              # a head without a scale; the row's others keep theirs
+    k[src[8]], v[src[8], -hd:] = 0, 0
+    slots, positions = [2, 0, 3, 1], [1, 4, 9, 0]
+    rows = KvRows(ints(starts_of(counts)), ints(positions), ints(slots), n_rows=total + pad, max_rows=max(counts),
+                  bad_flag=(flag := ints([0])))
+    K.kv_append_int8(cache, layer, rows, T(k), T(v), ints(list(src) + [10 ** 9] * pad) if gather else None)
+    back = [torch.full((total + pad, d), 7.0, device=DEV) for _ in range(4)]
+    K.kv_read_int8(back[0], back[1], cache, layer, rows)
+    K.kv_read_int8(back[2], None, cache, layer, rows)
+    K.kv_read_int8(None, back[3], cache, layer, rows)
+    assert H(flag)[0] == 0
+    for x, code, scale, outs in ((k, cache.k, cache.k_scales, back[::2]), (v, cache.v, cache.v_scales, back[1::2])):
+        lost = np.isnan(x[src])
+        q, s = quantize(np.where(lost, 0, x[src]), hd)
+        s[lost.reshape(total, n_kv, hd).any(2)] = np.nan
+        want_c, want_s = np.zeros(code.shape, np.int8), np.zeros(scale.shape, np.float32)
+        for i, (n, p, sl) in enumerate(zip(counts, positions, slots)):
+            r0 = starts_of(counts)[i]
+            want_c[sl, layer, p:p + n], want_s[sl, layer, p:p + n] = q[r0:r0 + n], s[r0:r0 + n]
+        assert np.array_equal(H(code), want_c) and np.array_equal(H(scale), want_s, equal_nan=True)
+        ref = (q.reshape(total, n_kv, hd).astype(np.float32) * s[..., None]).reshape(total, d)
+        for o in outs:
+            assert np.array_equal(H(o)[:total], ref, equal_nan=True) and (H(o)[total:] == 7).all()
