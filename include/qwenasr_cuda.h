@@ -296,7 +296,7 @@ typedef struct {
  * splits its work by it, results do not depend on it.  A sequence whose entries do
  * not fit (rows outside the packed buffers or the cache, more than max_rows
  * rows, a slot outside the cache) is left out, its outputs unwritten, and sets
- * *bad_flag (device, may be NULL; never cleared) to 1.  A call without
+ * *bad_flag (device, may be NULL; never cleared) to 1; the others are served.  A call without
  * sequences or rows does nothing, whatever its other pointers. */
 typedef struct {
   const int32_t *row_starts, *positions, *slots;

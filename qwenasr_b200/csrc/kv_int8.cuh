@@ -33,30 +33,29 @@ QASR_DEV KvSeq kv_seq(const qasr_kv_rows &r, const qasr_kv_int8 &c, int m) {
 }
 
 // Whole warp: where packed row `row` stands in the cache; ok = false for a row
-// behind the last sequence or of one that does not fit.  The owner is the last
-// sequence that starts at or below the row, found 32 at a time; its entries
-// come along in the same round of loads.  Starts in disorder give a sequence
-// that does not hold the row.
+// behind the last sequence or of one that does not fit.  Each lane takes the
+// entries of one sequence, checks them and sees whether they hold the row, so
+// that a bad start leaves out the sequences that it bounds and no others, as in
+// attention.  (Of sequences that overlap, which no good starts do, the first.)
 struct KvPlace {
   bool ok;
   int slot, pos;
 };
 QASR_DEV KvPlace kv_place(const qasr_kv_rows &r, const qasr_kv_int8 &c, int row, int lane) {
-  KvPlace at{false, 0, 0};
   for (int base = 0; base < r.n_seqs; base += 32) {
     const int i = base + lane;
     const bool in = i < r.n_seqs;
     const int start = in ? r.row_starts[i] : 0, end = in ? r.row_starts[i + 1] : 0, pos = in ? r.positions[i] : 0;
     const int slot = in && r.slots ? r.slots[i] : i;
-    const int below = __popc(__ballot_sync(0xffffffffu, in && start <= row));
-    if (below == 0) break;
-    const int own = below - 1;
-    const KvSeq s = kv_seq_checked(r, c, __shfl_sync(0xffffffffu, start, own), __shfl_sync(0xffffffffu, end, own),
-                                   __shfl_sync(0xffffffffu, pos, own), __shfl_sync(0xffffffffu, slot, own));
-    at = KvPlace{row >= s.row0 && row - s.row0 < s.n, s.slot, s.pos + (row - s.row0)};
-    if (below < 32) break;
+    const KvSeq s = kv_seq_checked(r, c, start, end, pos, slot);  // not in: without rows
+    const uint32_t hit = __ballot_sync(0xffffffffu, row >= s.row0 && row - s.row0 < s.n);
+    if (hit) {
+      const int own = __ffs(hit) - 1;
+      return KvPlace{true, __shfl_sync(0xffffffffu, s.slot, own),
+                     __shfl_sync(0xffffffffu, s.pos - s.row0, own) + row};
+    }
   }
-  return at;
+  return KvPlace{false, 0, 0};
 }
 
 // One warp of a launch: every sequence's entries, *bad_flag if one does not fit.

@@ -1,4 +1,4 @@
-"""The serving operators at their edges: scales that are no numbers, empty batches and lists, the variant of long calls."""
+"""The serving operators at their edges: scales that are no numbers, empty batches and lists, the variant of long calls, starts in disorder."""
 import numpy as np
 import pytest
 import torch
@@ -138,3 +138,37 @@ def test_long_calls(n_kv, hd, beyond, gather):
         ref = (q.reshape(total, n_kv, hd).astype(np.float32) * s[..., None]).reshape(total, d)
         for o in outs:
             assert np.array_equal(H(o)[:total], ref, equal_nan=True) and (H(o)[total:] == 7).all()
+
+
+# ------------------------------------------------------------- disorder --
+@pytest.mark.parametrize("starts,positions,fits", [
+    ([0, 50, 2, 4], [3, 0, 5], [2]),                     # a start outside leaves out the two sequences that it bounds
+    ([0, 2147483647, 2, 4, 6], [3, 0, 5, 1], [2, 3]),
+    ([0, 2, -9, 2, 4], [3, 0, 0, 5], [0, 3]),
+    ([0] + [2 * i + 2 for i in range(40)] + [200, 82, 84], [1] * 43, [*range(40), 42]),  # over a second ballot's lanes
+])
+def test_a_bad_start_leaves_the_others_in(starts, positions, fits):
+    """Every operator takes the same sequences: append and read-back write what attention attends for."""
+    rng = np.random.default_rng(len(starts))
+    n, n_rows, d = len(starts) - 1, max(s for s in starts if s < 100) + 2, 128
+    c = Cache(rng, n, 1, 16, 1, d)
+    for sl in range(n):
+        c.fill(rng, sl, 0, 16)
+    dev, flag = c.up(), ints([0])
+    rows = KvRows(ints(starts), ints(positions), None, n_rows=n_rows, max_rows=4, bad_flag=flag)
+    mine = np.zeros(n_rows, bool)
+    for m in fits:
+        mine[starts[m]:starts[m + 1]] = True
+    x = rng.standard_normal((n_rows, d)).astype(np.float32)
+    K.kv_append_int8(dev, 0, rows, T(x), T(x))
+    assert H(flag)[0] == 1
+    want = c.k.copy()
+    for m in fits:
+        r = starts[m + 1] - starts[m]
+        want[m, 0, positions[m]:positions[m] + r] = quantize(x[starts[m]:starts[m + 1]], d)[0]
+    assert np.array_equal(H(dev.k), want)
+    outs = [torch.full((n_rows, d), 9.0, device=DEV) for _ in range(2)]
+    K.kv_read_int8(outs[0], None, dev, 0, rows)
+    K.tree_attention_int8(outs[1], T(x), dev, 0, rows, 1, 0.1)
+    for o in outs:
+        assert np.array_equal((H(o) != 9).any(1), mine)
