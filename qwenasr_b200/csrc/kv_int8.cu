@@ -67,14 +67,15 @@ QASR_DEV uint32_t codes4(float4 x, float inv) {
   return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
+// The sources are plain pointers, here and in attention: what the kernel before writes, while this one's blocks are
+// resident already, must not go the way of read-only data.
 // Columns of a cache row go in pieces of 128 (one or two heads).  A warp takes
 // `per` pieces of one row, K and V; kPieces of each are in flight together.
 constexpr int kKvThreads = 128, kKvWarps = kKvThreads / 32;  // 32,640 rows: 58 us, 60 with 256 threads, 68 with 512
 template <int HD, int kPieces>
 __global__ void __launch_bounds__(kKvThreads)
-kv_append_int8_kernel(const qasr_kv_int8 c, int layer, const qasr_kv_rows r, const float *__restrict__ k_new,
-                      const float *__restrict__ v_new, const int32_t *__restrict__ src_rows, int n_src, int pieces,
-                      int per) {
+kv_append_int8_kernel(const qasr_kv_int8 c, int layer, const qasr_kv_rows r, const float *k_new, const float *v_new,
+                      const int32_t *src_rows, int n_src, int pieces, int per) {
   constexpr int LPH = HD / 4, HPP = 128 / HD;  // lanes per head, heads per piece
   const int lane = threadIdx.x & 31;
   const unsigned item = blockIdx.x * kKvWarps + (threadIdx.x >> 5), groups = (unsigned)(pieces + per - 1) / per;

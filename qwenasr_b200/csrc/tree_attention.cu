@@ -414,8 +414,8 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
 #pragma unroll
       for (int u = 0; u < HPB; ++u) {
         const bool in = more && next < len && (u == 0 || two);
-        nks[u] = in ? __ldg(ksp + u) : 0.0f;
-        nvs[u] = in ? __ldg(vsp + u) : 0.0f;
+        nks[u] = in ? ksp[u] : 0.0f;  // no read-only loads: the append before may have written them since the launch
+        nvs[u] = in ? vsp[u] : 0.0f;
       }
       next += kTaKeys;
       ksp += (size_t)kTaKeys * p.c.n_kv_heads;

@@ -172,3 +172,34 @@ def test_a_bad_start_leaves_the_others_in(starts, positions, fits):
     K.tree_attention_int8(outs[1], T(x), dev, 0, rows, 1, 0.1)
     for o in outs:
         assert np.array_equal((H(o) != 9).any(1), mine)
+
+
+# ---------------------------------------------------------------- order --
+def test_rows_written_just_before():
+    """Steps back to back, on two streams over one cache: each append's rows and scales, neighbours of those that the
+    attention before has read, are what the next attention sees (as with a wait after every call)."""
+    steps, d = 150, 128
+    rng = np.random.default_rng(3)
+    new = T(rng.standard_normal((2, steps, 3, 1, d)).astype(np.float32))
+    outs = []
+    for wait in (True, False):
+        cache, streams = KvCacheInt8.zeros(2, 1, 400, 1, d), [torch.cuda.Stream() for _ in range(2)]
+        out, pos = torch.zeros(2, steps, 1, d, device=DEV), [ints([0]) for _ in range(2)]
+        k, v = torch.empty(2, 1, d, device=DEV), torch.empty(2, 1, d, device=DEV)
+        rows = [KvRows(ints([0, 1]), pos[i], ints([i]), n_rows=1, max_rows=1, max_keys=400) for i in range(2)]
+        torch.cuda.synchronize()
+        for t in range(steps):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    pos[i].fill_(t)
+                    k[i].copy_(new[i, t, 0])
+                    v[i].copy_(new[i, t, 1])
+                    K.kv_append_int8(cache, 0, rows[i], k[i], v[i])
+                    if wait:
+                        torch.cuda.synchronize()
+                    K.tree_attention_int8(out[i, t], new[i, t, 2], cache, 0, rows[i], 1, 0.1)
+                    if wait:
+                        torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        outs.append(H(out))
+    assert np.array_equal(outs[0], outs[1]) and (outs[0] != 0).any(-1).all()
