@@ -352,10 +352,10 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
         umma_commit(&sm.empty[st]);
         umma_commit(&sm.ofull);
       }
-      if (!ok) {  // after a timeout: the products in flight end before TMEM is freed
-        umma_commit(&sm.done);
-        mbar_wait(&sm.done, 0);
-      }
+      // All products end before TMEM is freed, also where another role has given up and waits for none of them
+      // (otherwise the softmax warps wait for the last one meanwhile).
+      umma_commit(&sm.done);
+      mbar_wait(&sm.done, 0);
     }
   } else {
     // ------------------------------------------------------------ softmax
