@@ -248,13 +248,22 @@ __global__ void __launch_bounds__(kPickThreads, 2) logits_pick_kernel(const Pick
     key = s_warp[lane % kWarps];
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-    if (tid == 0) {
+    if (tid == 0)
       asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u64 [%0], %1, [%2];" ::"r"(
                        cluster_map(smem_u32(&s_rank[rank]), 0)),
                    "l"(key), "r"(cluster_map(smem_u32(&s_bar), 0))
                    : "memory");
-      if (rank == 0) {
-        const bool done = mbar_wait_cluster(&s_bar, 0);
+    if (rank == 0) {
+      bool done = __all_sync(0xffffffffu, mbar_wait_cluster(&s_bar, 0));
+      if (!done) {
+        // The others may yet send: this CTA must not leave before.  They wait for nothing and leave after it, and the
+        // cluster's barrier, which counts the threads that are left, then completes with this warp's arrival; what
+        // they sent lands soon after.  (The whole warp: a lane that has left the branch may wait for the others.)
+        cluster_arrive_all();
+        cluster_wait_all();
+        done = __all_sync(0xffffffffu, mbar_wait_cluster(&s_bar, 0));
+      }
+      if (tid == 0) {
         key = 0;
         for (int c = 0; c < (int)gridDim.x; ++c) key = max(key, *reinterpret_cast<volatile unsigned long long *>(&s_rank[c]));
         if (!done && r.bad_flag) atomicMax(r.bad_flag, -QASR_ERR_TIMEOUT);
