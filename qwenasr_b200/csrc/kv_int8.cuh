@@ -65,36 +65,6 @@ QASR_DEV void kv_flag_bad(const qasr_kv_rows &r, const qasr_kv_int8 &c, int lane
     if (!kv_seq(r, c, m).ok) atomicMax(r.bad_flag, 1);
 }
 
-// Two f32 in one register pair, two of a step at a time.
-using F2 = unsigned long long;
-QASR_DEV F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-QASR_DEV float f2_lo(F2 a) { return __uint_as_float((uint32_t)a); }
-QASR_DEV float f2_hi(F2 a) { return __uint_as_float((uint32_t)(a >> 32)); }
-QASR_DEV F2 f2_add(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-QASR_DEV F2 f2_add_up(F2 a, F2 b) {  // rounded up
-  F2 r;
-  asm("add.rp.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-QASR_DEV F2 f2_mul(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-QASR_DEV F2 f2_fma(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // Row (slot, layer, pos) of the cache, as an index of n_kv_heads scales.
 QASR_DEV size_t kv_row(const qasr_kv_int8 &c, int slot, int layer, int pos) {
   return ((size_t)slot * c.n_layers + layer) * c.max_seq + pos;

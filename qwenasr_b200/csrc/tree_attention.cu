@@ -106,6 +106,36 @@ QASR_DEV void tmem_ld_planes(uint32_t taddr, uint32_t stride, uint32_t (&d)[3][1
       : "memory");
 }
 
+// Two f32 in one register pair, two of a step at a time.
+using F2 = unsigned long long;
+QASR_DEV F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+QASR_DEV float f2_lo(F2 a) { return __uint_as_float((uint32_t)a); }
+QASR_DEV float f2_hi(F2 a) { return __uint_as_float((uint32_t)(a >> 32)); }
+QASR_DEV F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+QASR_DEV F2 f2_add_up(F2 a, F2 b) {  // rounded up
+  F2 r;
+  asm("add.rp.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+QASR_DEV F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+QASR_DEV F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 constexpr int kTaKeys = 128;             // keys of a tile: TMEM lanes of S^T
 constexpr int kTaTile = kTaKeys * 128;   // bytes of a K (or V) tile
 constexpr int kTaMaxCluster = 16;
@@ -381,8 +411,8 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       const uint32_t top = __reduce_max_sync(
           0xffffffffu, max(max(__float_as_uint(x.x) & kAbs, __float_as_uint(x.y) & kAbs),
                            max(__float_as_uint(x.z) & kAbs, __float_as_uint(x.w) & kAbs)));
-      // 2^e above the largest magnitude; below 2^-100 the scores are as good as zero.  NaN or an infinity
-      // (all exponent bits) makes the row's factor, and so its scores, NaN.
+      // 2^e above the largest magnitude; a row below 2^-100 loses bits.  NaN or an infinity (all exponent bits)
+      // makes the row's factor, and so its scores, NaN.
       const int r = warp + Sh::kWarps * k, e = max((int)(top >> 23) - 126, -100);
       ta_put_digits<NR>(sm.q, r, 4 * lane, x, __int_as_float((127 + 22 - e) << 23));
       if (lane == 0) {
