@@ -289,15 +289,16 @@ typedef struct {
  * when equal), which stand at rows positions[m] .. of cache slot slots[m]
  * (slots NULL: slot m).  row_starts [n_seqs + 1], positions and slots are
  * device arrays, read when the kernel runs, so a captured call follows their
- * contents (they must not change while a call runs).  n_rows: rows of the packed buffers; those from
- * row_starts[n_seqs] on are left as they are.  max_rows: at least the rows of
- * the longest sequence (it sizes the launch).  max_keys: how many cache rows
- * the longest sequence may have, if the host knows (0: max_seq); attention
- * splits its work by it, results do not depend on it.  A sequence whose entries do
- * not fit (rows outside the packed buffers or the cache, more than max_rows
- * rows, a slot outside the cache) is left out, its outputs unwritten, and sets
- * *bad_flag (device, may be NULL; never cleared) to 1; the others are served.  A call without
- * sequences or rows does nothing, whatever its other pointers. */
+ * contents (they must not change while a call runs).  n_rows: rows of the
+ * packed buffers; those from row_starts[n_seqs] on are left as they are.
+ * max_rows: at least the rows of the longest sequence (it sizes the launch).
+ * max_keys: how many cache rows the longest sequence may have, if the host
+ * knows (0: max_seq); attention splits its work by it, and results agree to
+ * rounding whatever it is.  A sequence whose entries do not fit (rows outside
+ * the packed buffers or the cache, more than max_rows rows, a slot outside the
+ * cache) is left out, its outputs unwritten, and sets *bad_flag (device, may be
+ * NULL; never cleared) to 1; the others are served.  A call without sequences
+ * or rows does nothing, whatever its other pointers. */
 typedef struct {
   const int32_t *row_starts, *positions, *slots;
   int n_seqs, n_rows, max_rows, max_keys;
@@ -327,7 +328,7 @@ int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 *cache, int
  * 0 .. positions[m]-1, and of the rows positions[m] + j, which hold the K/V of
  * its own tokens (append them first), those that tree_mask allows: token t
  * sees row j when bit j of tree_mask[row_starts[m] + t] is set (device,
- * [n_rows]; sequences of at most 64 rows).  tree_mask NULL: j <= t, the
+ * [n_rows]; max_rows at most 64).  tree_mask NULL: j <= t, the
  * causal rule of qasr_causal_attention; with one row per sequence this is a
  * decode step, with many a prompt chunk.  out [n_rows, n_heads * head_dim] =
  * softmax(scale * q k^T) v in f32; a row that sees nothing is zero, one that
@@ -336,9 +337,9 @@ int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 *cache, int
  * beyond the range of f32 is an infinity: -infinity weighs nothing, +infinity
  * makes NaN.  A query row is rounded to 23 bits of its largest magnitude, the
  * products of weight and value scale to 23 bits of the largest one that the row
- * sees among 128 keys; sums are 32-bit or f32.  n_heads a multiple of
- * n_kv_heads, at most 64 query heads per kv head; q and out 16-byte aligned
- * and without overlap.  No workspace: calls may run at once on any streams.
+ * sees among 128 keys (both of 2^-100 at least); sums are 32-bit or f32.  n_heads a multiple of
+ * n_kv_heads, at most 64 query heads per kv head, at most 65,535 sequences; q
+ * and out 16-byte aligned and without overlap.  No workspace: calls may run at once on any streams.
  * If a bounded device-side wait gives up, *bad_flag becomes -QASR_ERR_TIMEOUT
  * and the rows concerned are NaN. */
 int qasr_tree_attention_int8(float *out, const float *q, const qasr_kv_int8 *cache, int layer,
@@ -371,7 +372,10 @@ typedef struct {
  *   then plus its bias; a token that allow_mask does not allow becomes -inf.
  * logits_out [M, vocab] (NULL, or logits itself, or disjoint from it) receives
  * the values and ids [M] (may be NULL if logits_out is not) the first largest
- * allowed one, NaN aside; -1 when there is none. */
+ * allowed one, NaN aside; -1 when there is none.  All three penalties go by one
+ * history; over two of them (repetition over prompt and output, the others over
+ * the output) it takes two calls: repetition into logits_out without ids, then
+ * the rest in place.  At most 65,535 rows and 2^30 tokens. */
 int qasr_logits_pick(int32_t *ids, float *logits_out, const float *logits, const qasr_pick_rules *rules, int M,
                      int vocab, void *stream);
 

@@ -341,7 +341,9 @@ def logits_pick(ids_out, logits_out, logits, M, vocab, history=None, history_sta
     """Penalties of repeated tokens, biases and the mask of allowed tokens on
     logits [M, vocab], then the first-max pick (qasr_logits_pick).  ids_out or
     logits_out may be None; logits_out may be logits.  Lists are packed with
-    starts [M + 1] and may be empty; allow_mask is int32 [M, ceil(vocab / 32)], bit set = allowed."""
+    starts [M + 1] and may be empty; the three penalties share the history (two
+    histories: two calls, the second in place); allow_mask is int32
+    [M, ceil(vocab / 32)], bit set = allowed."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
     dev = logits.get_device()

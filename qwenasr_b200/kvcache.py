@@ -63,7 +63,7 @@ class KvRows:
     kernels run: they may be changed in place between calls or graph replays.
     n_rows: rows of the packed buffers; max_rows: a bound on one sequence's
     rows; max_keys: a bound on one sequence's cache rows, by which attention
-    splits its work (0: the cache's max_seq); bad_flag: int32 [1], set when a
+    splits its work (0: the cache's max_seq; results agree to rounding); bad_flag: int32 [1], set when a
     sequence does not fit."""
 
     def __init__(self, row_starts: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor | None = None, *,

@@ -1,10 +1,11 @@
-"""The serving operators at their edges: scales that are no numbers, empty batches and lists, the variant of long calls, starts in disorder."""
+"""The serving operators at their edges: scales that are no numbers, empty batches and lists, the variant of long calls,
+starts in disorder, rows written just before, penalties over two histories."""
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_serving import (Cache, DEV, H, KvCacheInt8, KvRows, T, as_int64, attend_exact, ints, pack, pick_ref,
-                              quantize, starts_of)
+from test_gpu_serving import (Cache, DEV, H, KvCacheInt8, KvRows, T, as_int64, attend_exact, ints, mask_words, pack,
+                              pick_ref, quantize, starts_of)
 
 from qwenasr_b200 import kernels as K
 
@@ -203,3 +204,26 @@ def test_rows_written_just_before():
         torch.cuda.synchronize()
         outs.append(H(out))
     assert np.array_equal(outs[0], outs[1]) and (outs[0] != 0).any(-1).all()
+
+
+# --------------------------------------------------------- two histories --
+def test_penalties_over_two_histories():
+    """Repetition over prompt and output, presence and frequency over the output alone: two calls, the second in
+    place, give what the rule says for both lists."""
+    rng = np.random.default_rng(4)
+    M, V = 3, 900
+    x = (rng.standard_normal((M, V)) * 3).astype(np.float32)
+    prompt = [list(rng.integers(0, V, 60)) for _ in range(M)]
+    output = [[], list(rng.integers(0, V, 5)), list(rng.integers(0, 9, 40))]
+    rep, pres, freq = (rng.random(M).astype(np.float32) + b for b in (np.float32(1), np.float32(0), np.float32(0)))
+    one, zero = np.ones(M, np.float32), np.zeros(M, np.float32)
+    allow = rng.random((M, V)) < 0.7
+    _, mid = pick_ref(x, [p + o for p, o in zip(prompt, output)], rep, zero, zero, None, None)
+    ref_ids, ref = pick_ref(mid, output, one, pres, freq, None, allow)
+    ids, out = ints([-7] * M), torch.empty(M, V, device=DEV)
+    h, s = pack([p + o for p, o in zip(prompt, output)])
+    K.logits_pick(None, out, T(x), M, V, history=h, history_starts=s, repetition=T(rep))
+    h, s = pack(output)
+    K.logits_pick(ids, out, out, M, V, history=h, history_starts=s, presence=T(pres), frequency=T(freq),
+                  allow_mask=mask_words(allow, V))
+    assert np.array_equal(H(ids), ref_ids) and np.array_equal(H(out), ref)
