@@ -335,9 +335,9 @@ int qasr_kv_read_int8(float *k_out, float *v_out, const qasr_kv_int8 *cache, int
  * sees a scale of NaN or infinity (or a value scale below 0 or from 2^125 on) is
  * NaN, and so is the row of a query holding either that sees anything.  A score
  * beyond the range of f32 is an infinity: -infinity weighs nothing, +infinity
- * makes NaN.  A query row is rounded to 23 bits of its largest magnitude, the
- * products of weight and value scale to 23 bits of the largest one that the row
- * sees among 128 keys (both of 2^-100 at least); sums are 32-bit or f32.  n_heads a multiple of
+ * makes NaN.  A query row is rounded to 24 bits of its largest magnitude (half
+ * a per cent of rows: 23), the products of weight and value scale to 23 bits of
+ * the largest one that the row sees among 128 keys (both of 2^-100 at least); sums are 32-bit or f32.  n_heads a multiple of
  * n_kv_heads, at most 64 query heads per kv head, at most 65,535 sequences; q
  * and out 16-byte aligned and without overlap.  No workspace: calls may run at once on any streams.
  * If a bounded device-side wait gives up, *bad_flag becomes -QASR_ERR_TIMEOUT

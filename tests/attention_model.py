@@ -6,8 +6,9 @@ Codes kc, vc [n, hd], scales ks, vs [n], `see` [n] the keys the row may see.
 
 The bar.  Let w_j = e^(s_j - max), u_j = w_j * vs_j, L = sum w_j, o = sum u_j vc_j / L over the visible keys.
 What the kernel rounds, and how far that moves o:
-* q: 23 bits of the row's largest magnitude, half a step h = 2^(E - 23), 2^E above it: s_j moves by scale * ks_j
-  times sum_d dq_d kc_jd, of variance (h^2 / 3) |kc_j|^2; o moves by sum_j (u_j vc_j - w_j o) ds_j / L.
+* q: half a step h = 2^(E - 24), 2^E above the row's largest magnitude (2^(E - 23) for the few largest magnitudes
+  that pass three digits): s_j moves by scale * ks_j times sum_d dq_d kc_jd, of variance (h^2 / 3) |kc_j|^2; o moves
+  by sum_j (u_j vc_j - w_j o) ds_j / L.
 * the scores' f32 steps (8 roundings of the score) and the exponential (2^-22): the same sum, each key on its own.
 * u_j, half a unit of 2^-22.99 of the largest u_j in its tile of 128 keys: variance (unit^2 / 12) |vc_j|^2 / L^2;
   and 3 roundings of its own.
@@ -32,7 +33,8 @@ def exact(q, kc, ks, vc, vs, scale, see):
     w = np.exp(s - s.max())
     u, L = w * vs, w.sum()
     o = u @ vc / L
-    h = 2.0 ** (np.ceil(np.log2(np.abs(q).max())) - 23) if np.abs(q).max() > 0 else 0.0
+    top, e = np.frexp(np.abs(q).max())
+    h = 2.0 ** (e - 24.0 + (np.rint(top * 2.0 ** 23) > 127 * 65793))
     size = np.linalg.norm(vc, axis=1)
     lean = np.linalg.norm(u[:, None] * vc - w[:, None] * o, axis=1)
     ds2 = (scale * ks * h) ** 2 / 3 * (kc ** 2).sum(1) + (8 * 2.0 ** -24 * s) ** 2 + 2.0 ** -44
@@ -53,10 +55,11 @@ def model(q, kc, ks, vc, vs, scale, see, per_row=True, lose=None):
     q, ks, vs = q.astype(f), ks.astype(f), vs.astype(f)
     top = np.abs(q).max()
     e = int(np.frexp(top)[1]) if top > 0 else -100
-    X = np.rint(np.ldexp(q, 22 - e)).astype(np.int64)
+    up = 23 - e - (int(np.rint(np.ldexp(top, 23 - e))) > 127 * 65793)  # what three signed digits hold
+    X = np.rint(np.ldexp(q, up)).astype(np.int64)
     if lose == "q":
         X = (X + 128) // 256 * 256
-    qf = f(np.ldexp(f(1), e - 22)) * (f(scale) * f(1.44269504))
+    qf = f(np.ldexp(f(1), -up)) * (f(scale) * f(1.44269504))
     x = (kc.astype(np.int64) @ X).astype(f) * (qf * ks)
     x = np.where(see, x, f(-np.inf))
     n = len(x)
