@@ -44,8 +44,8 @@ QASR_DEV void pick_fit(int n, int &a, int &b, int32_t *bad) {
 // maxima are kept on the way; the token is looked up by the few threads that
 // hold the CTA's maximum.  Every CTA sends its best to rank 0 with a store that
 // counts on a barrier there and leaves: nobody waits for its own output.
-// Measured (B200, 151,936 tokens): one row with a history of 120 3.9 us (launch
-// and two round trips), 8 rows 4.7, 64 rows with every rule 23.0 us, 3.4 TB/s
+// Measured (B200, 151,936 tokens): one row with a history of 120 4.1 us (launch
+// and two round trips), 8 rows 4.9, 64 rows with every rule 23.2 us, 3.4 TB/s
 // (loads, instructions and stores of four tiles one after the other; 18 us
 // without mask and bias).
 // VEC: rows start on 16-byte boundaries; a quad is four neighbours, loaded as

@@ -41,11 +41,13 @@
 // workspace, no atomics and no second launch.
 //
 // Measured (B200, 16 query heads over 8 kv heads of 128, calls replayed back to
-// back): 32 sequences x 1 token over 8000 keys 81.6 us, 541 MB, the copy rate
-// (HBM-bound); over 250 .. 8000 keys 47.8 us; one sequence over 545 keys 4.9 us (the
-// chain of one tile); 8 trees of 31 tokens 15.5 us and prompts of 4 x 404 tokens 22.8 us
-// (about 37 softmax instructions per query row and key, half of the issue slots;
-// the tensor pipe is busy 15 % of the time).
+// back): 32 sequences x 1 token over 8000 keys 87 us, 541 MB, 0.95 of the copy
+// rate (HBM-bound); over 250 .. 8000 keys 47.4 us; one sequence over 545 keys 5.1 us
+// (the chain of one tile), 8 over 1001 keys 6.5 us; 8 trees of 31 tokens 16.6 us
+// (256 CTAs in one wave: the longest history's five tiles in one CTA, where the
+// mean is 2.75, and the set-up and exchange around them); prompts of 4 x 404 tokens
+// 24.3 us (728 CTAs with work in 2.5 waves, two tiles each on average; all
+// instructions together, 75 per query row and key, are 12 us of issue).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -729,7 +731,8 @@ static int tree_attention_launch(TreeAttnParams p, cudaStream_t st) {
   // long histories (32 tiles) may differ in length and the longest would set the time: 256 blocks over 250 .. 8000 rows
   // take 47 us with two each and 62 with one (all 8000: 87 and 81); 128 blocks 30 with four and 36 with two (50 and
   // 44).  Sixteen of a cluster find room on few SMs of a GPC at a time: only for 8 blocks (2000 rows: 5.6 us, 5.7 with
-  // 8; 16 blocks 9.4 and 5.5).
+  // 8; 16 blocks 9.4 and 5.5).  These are single tokens; blocks of 32 rows go by the same limits.  Without a bound
+  // from the host the tiles are the cache's capacity, and short histories in a large cache get CTAs without work.
   const int keys = p.r.max_keys > 0 ? std::min(p.r.max_keys, p.c.max_seq) : p.c.max_seq;
   const int tiles = ceil_div(keys, kTaKeys);
   const long blocks = (long)heads * row_blocks * p.r.n_seqs;
