@@ -552,16 +552,31 @@ tree_attention_kernel(const __grid_constant__ TreeAttnParams p) {
       // A product's integer is 2^(x - base) * vs * units, at most 2^23: 2^22.998 leaves room for the errors of the
       // logarithms and exponentials (below 2^-13 in all) and for the roundings.  What a unit counts is the reciprocal
       // of `units`, to an ulp or two that scales the whole tile's share.
-      const float most = lane < 2 * R ? over_warps(lane) : 0.0f, umax = __shfl_down_sync(0xffffffffu, most, R);
+      const float most = lane < 2 * R ? over_warps(lane) : 0.0f;
+      float umax = __shfl_down_sync(0xffffffffu, most, R);
+      const float top = fmaxf(m_run, most), base = lane >= R || top == -INFINITY ? 0.0f : top;
+      float *c = reinterpret_cast<float *>(sm.rowc[buf][warp][lane / 2 % (R / 2)]) + lane % 2;
+      if (lane < R) c[0] = -base;
+      umax = __fsub_rn(umax, base);
+      // Where scores are so large that a product's logarithm, rounded up, says little, the logarithms are taken again,
+      // less the base.  All warps of the group have the same bases: they all come here, or none.
+      if (__any_sync(0xffffffffu, fabsf(base) >= 65536.0f)) {
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < R; r += 2) {
+          const F2 from = f2_add(f2(x[r], x[r + 1]), sm.rowc[buf][warp][r / 2][0]);
+          const F2 y = f2_add_up(from, f2(of_row(lvs, r), of_row(lvs, r + 1)));
+          const float2 u2 = make_float2(ta_warp_max(f2_lo(y)), ta_warp_max(f2_hi(y)));
+          if (lane == 0) *reinterpret_cast<float2 *>(&sm.wmax[buf][warp][R + r]) = u2;
+        }
+        named_bar(2 + wg, 128);
+        if (lane < R) umax = over_warps(R + lane);
+      }
       if (lane < R) {
-        const float top = fmaxf(m_run, most), base = top == -INFINITY ? 0.0f : top;
-        const float old = m_run == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(m_run, base));
         // a tile whose products are all below 2^-100 of the row's largest weight loses bits
-        const float units = ta_ex2(__fadd_rn(fminf(__fsub_rn(base, umax), 100.0f), 22.998f));
-        float *c = reinterpret_cast<float *>(sm.rowc[buf][warp][lane / 2]) + lane % 2;
-        c[0] = -base;
+        const float units = ta_ex2(__fadd_rn(fminf(-umax, 100.0f), 22.998f));
         c[2] = units;
-        c[4] = old;
+        c[4] = m_run == -INFINITY ? 0.0f : ta_ex2(__fsub_rn(m_run, base));
         c[6] = ta_rcp(units);
         m_run = top;
       }

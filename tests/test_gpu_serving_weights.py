@@ -69,3 +69,61 @@ def test_rows_by_norm(kind, counts, positions, n_kv, group, hd, tree, max_keys):
                                  c.vs[i, 0, :p + r, kv], scale, see)
                 err = np.linalg.norm(got[row, h] - o)
                 assert err <= bar, (i, t, h, err / bar, err / np.linalg.norm(o))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("power", [0, 10, 20, 24, 26, 29, 32, 40, 70])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_every_size(power, hd, sign):
+    """One key's score is far from the others', at 2^power: beyond 2^24 f32 holds the scores' own differences coarsely,
+    and the result is that key's value row to the bits that a product keeps (2^-22 of it, and 4 roundings), whatever
+    the value scales are; with equal scores it is the mean."""
+    rng = np.random.default_rng(power)
+    n, n_kv, group = 300, 2, 9                        # 18 rows a kv head: a block of 32
+    c = Cache(rng, 1, 1, 400, n_kv, hd)
+    c.fill(rng, 0, 0, n)
+    win, s = 170, hd ** -0.5
+    c.k[0, 0, :n] = 1 if sign > 0 else 3              # the winner's score: 2^power * 3, or -2^power among -3 * 2^power
+    c.k[0, 0, win] = 3 if sign > 0 else 1
+    c.ks[0, 0, :n] = np.float32(sign * 2.0 ** power / (hd * s))
+    c.vs[0, 0, :n] *= np.exp2(rng.integers(-9, 10, (n, n_kv))).astype(np.float32)
+    c.vs[0, 0, win] = [3.7, 0.02]
+    q = np.ones((1, n_kv * group * hd), np.float32)
+    out = torch.empty(1, n_kv * group * hd, device=DEV)
+    for max_keys in (0, 1):
+        rows = KvRows(ints([0, 1]), ints([n - 1]), n_rows=1, max_rows=1, max_keys=max_keys)
+        K.tree_attention_int8(out, T(q), c.up(), 0, rows, n_kv * group, s)
+        got = H(out).reshape(n_kv, group, hd).astype(np.float64)
+        for kv in range(n_kv):
+            cut = slice(kv * hd, (kv + 1) * hd)
+            o, bar = A.exact(q[0, :hd], c.k[0, 0, :n, cut], c.ks[0, 0, :n, kv], c.v[0, 0, :n, cut], c.vs[0, 0, :n, kv],
+                             s, np.ones(n, bool))
+            if power >= 10:                           # the others weigh e^-2048 or nothing
+                o = c.v[0, 0, win, cut] * np.float64(c.vs[0, 0, win, kv])
+                bar = (2.0 ** -22 + 4 * 2.0 ** -24) * np.linalg.norm(o)
+            assert (np.linalg.norm(got[kv] - o, axis=1) <= bar).all(), (power, np.linalg.norm(got[kv] - o, axis=1) / bar)
+
+
+@pytest.mark.parametrize("power", [-90, -40, 40, 105])
+@pytest.mark.parametrize("hd,group", [(128, 2), (128, 20), (64, 1), (64, 9)])
+def test_values_of_every_size(power, hd, group):
+    """All value scales at 2^power: the result scales with them, to the bar of ordinary values."""
+    rng = np.random.default_rng(hd + group)
+    n = 700
+    c = Cache(rng, 1, 1, 900, 2, hd)
+    q = np.empty((2, group, hd), np.float32)
+    for kv in range(2):
+        cut = slice(kv * hd, (kv + 1) * hd)
+        q0, c.k[0, 0, :n, cut], c.ks[0, 0, :n, kv], c.v[0, 0, :n, cut], c.vs[0, 0, :n, kv] = A.history(rng, "plain", n, hd)
+        q[kv] = q0 * (1 + 0.1 * rng.standard_normal((group, hd)))
+    c.vs[0, 0, :n] *= np.float32(2.0 ** power)
+    out = torch.empty(1, 2 * group * hd, device=DEV)
+    rows = KvRows(ints([0, 1]), ints([n - 1]), n_rows=1, max_rows=1)
+    K.tree_attention_int8(out, T(q.reshape(1, -1)), c.up(), 0, rows, 2 * group, hd ** -0.5)
+    got = H(out).reshape(2, group, hd).astype(np.float64)
+    for kv in range(2):
+        cut = slice(kv * hd, (kv + 1) * hd)
+        for h in range(group):
+            o, bar = A.exact(q[kv, h], c.k[0, 0, :n, cut], c.ks[0, 0, :n, kv], c.v[0, 0, :n, cut], c.vs[0, 0, :n, kv],
+                             hd ** -0.5, np.ones(n, bool))
+            assert np.linalg.norm(got[kv, h] - o) <= bar
